@@ -15,6 +15,8 @@ OK, ERR_INVALID_ARG, ERR_BAD_ALIGNMENT, ERR_CUDA, ERR_TIMEOUT, ERR_UNSUPPORTED, 
 NVFP4_SPEC, NVFP4_KERNEL_IEEE, NVFP4_KERNEL_FAST = 0, 1, 2
 GEMM_DEFAULT, GEMM_PAIR_N256, GEMM_SINGLE_N256, GEMM_PAIR_N128, GEMM_SINGLE_N128, GEMM_SKINNY, GEMM_SKINNY_PREFETCH, GEMM_PAIR_M512_N256 = range(8)
 
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = range(3)
+
 
 class TkbError(RuntimeError):
     def __init__(self, code: int, message: str):
@@ -76,6 +78,11 @@ _SIGNATURES = {
     "tkb_fp8_gemm": ([_vp, _i64, _vp, _i64, _vp, _i64, _i, _i, _i, _vp], _i),
     "tkb_fp8_gemm_ex": ([_vp, _i64, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _vp], _i),
     "tkb_nvfp4_gemm_quant": ([_vp] * 10 + [_i, _i, _i, _i, _vp], _i),
+    "tkb_int8_quantize": ([_vp, _i64, _i, _vp, _i64, _vp, _i, _i, _vp], _i),
+    "tkb_rms_norm": ([_vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _i, _i, _i, C.c_float, _vp], _i),
+    "tkb_block_norm": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i, C.c_float, _vp, _vp, _i64, _vp, _i64, _vp, _i, _i, _i, C.c_float, _vp], _i),
+    "tkb_int8_gemm": ([_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _vp], _i),
+    "tkb_int8_gemm_ex": ([_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _i, _vp], _i),
     "tkb_bf16_gemm_ex": ([_vp, _i64, _vp, _i64, _vp, _i64, _i, _i, _i, _i, _vp], _i),
 }
 

@@ -34,6 +34,7 @@ constexpr int kQuantSlots = 256;
 constexpr int kDecodeRing = 4;                           // streams of one device that may use the skinny-M GEMM
 constexpr int kSmallScratchRing = 4;
 constexpr size_t kSmallScratchBytes = 2u << 20;
+constexpr int kInt8MaxK = 131071;                        // 128 * 128 * K < 2^31
 constexpr int kDecodeMaxGrid = 160;                      // CTAs the scratch is sized for
 constexpr size_t kDecodePartialFloats = size_t(kDecodeMaxGrid) * 128 * 128;
 
@@ -200,7 +201,18 @@ static int pick_config(int kind, int config, int M, int N, int sm_count) {
     return 2;
 }
 
-// bf16 output map: box 64 columns x 32 rows, 128-byte swizzle (one epilogue warp's staging box)
+// fp32 output map: box 32 columns x 32 rows, 128-byte swizzle (one epilogue warp's staging box)
+static int make_output_map_fp32(CUtensorMap* m, void* D, int rows, int cols, int64_t ldd) {
+    cuuint64_t dims[2] = {uint64_t(cols), uint64_t(rows)};
+    cuuint64_t strides[1] = {uint64_t(ldd) * 4};
+    cuuint32_t box[2] = {32, 32};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, D, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return api_fail(TKB_ERR_CUDA, "cuTensorMapEncodeTiled(fp32 output) failed with CUresult %d", int(r));
+    return TKB_OK;
+}
+// bf16 (or any 16-bit) output map: box 64 columns x 32 rows, 128-byte swizzle
 int api_make_output_map(CUtensorMap* m, void* D, int rows, int cols, int64_t ldd) {
     cuuint64_t dims[2] = {uint64_t(cols), uint64_t(rows)};
     cuuint64_t strides[1] = {uint64_t(ldd) * 2};
@@ -306,6 +318,50 @@ static int gemm_common(int kind, const void* A, int64_t lda_bytes, const void* A
     g.config = pick_config(kind, config, M, N, c->sm_count);
     if (int e = api_make_gemm_maps(&g, kind, A, lda_bytes, A_sc, B, ldb_bytes, B_sc, D, ldd, M, N, K)) return e;
     g.sgA = A_sg; g.sgB = B_sg; g.M = M; g.N = N; g.K = K;
+    g.status = c->status; g.prof = g_prof; g.sm_count = c->sm_count; g.stream = static_cast<cudaStream_t>(stream);
+    TKB_CUDA(launch_gemm(g));
+    return TKB_OK;
+}
+
+// D = (A_sc x B_sc) * (A . B^T) with int8 operands
+static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const void* B, int64_t ldb, const float* B_sc, void* D, int64_t ldd, int dtype,
+                            int M, int N, int K, int config, void* stream) {
+    if (dtype != TKB_DTYPE_BF16 && dtype != TKB_DTYPE_FP16 && dtype != TKB_DTYPE_FP32) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: unknown output dtype %d", dtype);
+    if (M < 0 || N < 1 || K < 1) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: need M >= 0 and N, K >= 1 (got %d, %d, %d)", M, N, K);
+    if (K > kInt8MaxK) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: K=%d is above %d, where a sum of K products may leave int32", K, kInt8MaxK);
+    if (config < TKB_GEMM_DEFAULT || config > TKB_GEMM_SINGLE_N128) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: config %d is not a tile of this format", config);
+    if (lda == 0) lda = K;
+    if (ldb == 0) ldb = K;
+    if (ldd == 0) ldd = N;
+    if (lda < K || ldb < K || ldd < N) return api_fail(TKB_ERR_BAD_ALIGNMENT, "int8_gemm: lda, ldb must be >= K and ldd >= N");
+    if (M == 0) return TKB_OK;
+    if (!A || !A_sc || !B || !B_sc || !D) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: null pointer");
+    // a single row has no pitch that anything reads
+    if (M == 1) lda = (int64_t(K) + 15) / 16 * 16;
+    if (N == 1) ldb = (int64_t(K) + 15) / 16 * 16;
+    if (!aligned16(A) || !aligned16(B) || lda % 16 || ldb % 16)
+        return api_fail(TKB_ERR_BAD_ALIGNMENT, "int8_gemm: operand base pointers and row pitches must be multiples of 16 bytes (lda=%lld ldb=%lld); rows of odd K need padded pitches",
+                        (long long)lda, (long long)ldb);
+    const int out_bytes = dtype == TKB_DTYPE_FP32 ? 4 : 2;
+    if ((reinterpret_cast<uintptr_t>(A_sc) | reinterpret_cast<uintptr_t>(B_sc)) & 3u || reinterpret_cast<uintptr_t>(D) & uintptr_t(out_bytes - 1))
+        return api_fail(TKB_ERR_BAD_ALIGNMENT, "int8_gemm: scales and D must be aligned to their element type");
+    DeviceCtx* c;
+    if (int e = get_ctx(&c)) return e;
+    GemmArgs g;
+    memset(&g, 0, sizeof(g));
+    g.kind = KIND_INT8;
+    g.config = pick_config(KIND_INT8, config, M, N, c->sm_count);
+    const int ctas = (g.config & 1) ? 1 : 2;
+    if (int e = make_operand_map(&g.tmA, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, lda, 128)) return e;
+    if (int e = make_operand_map(&g.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, ldb, gemm_tile_n(g.config) / ctas)) return e;
+    g.tmSA = g.tmA; g.tmSB = g.tmB; g.tmD = g.tmA;
+    g.plain_out = !aligned16(D) || (M > 1 && ldd * out_bytes % 16);
+    if (!g.plain_out) {
+        const int64_t pitch = M > 1 ? ldd : (int64_t(N) + 7) / 8 * 8;
+        if (int e = dtype == TKB_DTYPE_FP32 ? make_output_map_fp32(&g.tmD, D, M, N, pitch) : api_make_output_map(&g.tmD, D, M, N, pitch)) return e;
+    }
+    g.out_dtype = dtype; g.D = D; g.ldd = ldd;
+    g.sgA = A_sc; g.sgB = B_sc; g.M = M; g.N = N; g.K = K;
     g.status = c->status; g.prof = g_prof; g.sm_count = c->sm_count; g.stream = static_cast<cudaStream_t>(stream);
     TKB_CUDA(launch_gemm(g));
     return TKB_OK;
@@ -567,6 +623,15 @@ int tkb_fp8_gemm_ex(const void* A, int64_t lda, const void* B, int64_t ldb, void
 }
 int tkb_fp8_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, void* D, int64_t ldd, int M, int N, int K, void* stream) {
     return tkb_fp8_gemm_ex(A, lda, B, ldb, D, ldd, M, N, K, TKB_GEMM_DEFAULT, stream);
+}
+
+int tkb_int8_gemm_ex(const void* A, int64_t lda, const float* A_sc, const void* B, int64_t ldb, const float* B_sc, void* D, int64_t ldd, int dtype,
+                     int M, int N, int K, int config, void* stream) {
+    return int8_gemm_common(A, lda, A_sc, B, ldb, B_sc, D, ldd, dtype, M, N, K, config, stream);
+}
+int tkb_int8_gemm(const void* A, int64_t lda, const float* A_sc, const void* B, int64_t ldb, const float* B_sc, void* D, int64_t ldd, int dtype,
+                  int M, int N, int K, void* stream) {
+    return int8_gemm_common(A, lda, A_sc, B, ldb, B_sc, D, ldd, dtype, M, N, K, TKB_GEMM_DEFAULT, stream);
 }
 
 } // extern "C"

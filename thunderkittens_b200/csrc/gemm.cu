@@ -6,6 +6,8 @@
 //                (replaces mxfp8_gemm::kernel, kernels/gemm/mxfp8_b200/mxfp8_b200_gemm.cu:83-292)
 //   KIND_BF16  : dense control (replaces kernel<C>, kernels/gemm/bf16_b200/bf16_b200_gemm.cu:61-253)
 //   KIND_FP8   : dense e4m3 (replaces kernels/gemm/fp8_b200/fp8_b200_gemm.cu, the bf16 kernel with 8-bit operands)
+//   KIND_INT8  : int8, exact int32 accumulation, one fp32 scale per row of A and per row of B applied in the epilogue; D is
+//                bf16, fp16 or fp32 (no counterpart in the reference)
 //
 // Design (one CTA per SM, persistent over output tiles):
 //   * A stage of the operand ring always holds exactly 128 bytes of K per row (64 bf16, 128 e4m3,
@@ -35,6 +37,7 @@
 #include "ptx.cuh"
 #include "internal.h"
 #include "ag_schedule.h"
+#include "../../include/tkb200.h"
 
 namespace tkb {
 
@@ -92,6 +95,8 @@ struct GemmParams {
     uint8_t* q_codes; uint8_t* q_sc; float* q_sg; const float* q_amax; int q_arith;
     // reduce-scatter epilogue (MODE_RS): tensor maps (device memory) of every rank's output rows, rows per rank
     const CUtensorMap* rs_maps; int rs_rows;
+    // KIND_INT8: output type and, for outputs that TMA cannot address, where to store without it
+    int out_dtype, plain_out; void* D; int64_t ldd;
 };
 
 // NVFP4 quantization of one 16-value block held as 8 packed bf16 pairs, with the IEEE arithmetic of the standalone
@@ -120,6 +125,87 @@ __device__ __forceinline__ uint8_t quant_block16(const uint32_t (&w)[8], float s
     }
     codes = make_uint2(out[0], out[1]);
     return s8;
+}
+
+// Epilogue of KIND_INT8 for one warp: 32 rows x 64 columns of int32 sums (this thread: row row0 + lane) are scaled, converted
+// and leave through the warp's staging box (rows of 128 bytes, 128-byte swizzle): one box of 64 columns for the 16-bit types,
+// two of 32 columns for fp32.  The sums are converted to fp32 first (one rounding above 2^24), then multiplied by the row's and
+// by the column's scale.  A box leaves by TMA, which clips the edges of D, or, where D's base or pitch is not a multiple of 16
+// bytes, row by row with one element per lane.
+__device__ __forceinline__ void int8_epilogue(uint32_t (&r)[64], const CUtensorMap* tmD, const GemmParams& p, uint32_t stage_box, int row0, int col0,
+                                              float row_scale, int lane, uint64_t policy) {
+    if (row0 >= p.M || col0 >= p.N) return;                  // uniform over the warp
+    const float* cs = p.sgB + col0;
+    if (col0 + 64 <= p.N && (reinterpret_cast<uintptr_t>(cs) & 15u) == 0) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float4 c = __ldg(reinterpret_cast<const float4*>(cs) + i);      // the same address in all lanes
+            r[4 * i] = __float_as_uint(__int2float_rn(int(r[4 * i])) * row_scale * c.x);
+            r[4 * i + 1] = __float_as_uint(__int2float_rn(int(r[4 * i + 1])) * row_scale * c.y);
+            r[4 * i + 2] = __float_as_uint(__int2float_rn(int(r[4 * i + 2])) * row_scale * c.z);
+            r[4 * i + 3] = __float_as_uint(__int2float_rn(int(r[4 * i + 3])) * row_scale * c.w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 64; i++) r[i] = __float_as_uint(__int2float_rn(int(r[i])) * row_scale * __ldg(cs + min(i, p.N - 1 - col0)));
+    }
+    auto leave = [&](int col, int elem_bytes) {              // the box holds columns col .. col + 128 / elem_bytes - 1
+        if (!p.plain_out) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d_hint(tmD, stage_box, col, row0, policy);
+                tma_store_commit();
+            }
+            return;
+        }
+        __syncwarp();
+        const int rows = min(32, p.M - row0);
+        for (int row = 0; row < rows; row++) {
+            uint8_t* out = static_cast<uint8_t*>(p.D) + (int64_t(row0 + row) * p.ldd + col) * elem_bytes;
+            for (int e = lane; e < 128 / elem_bytes && col + e < p.N; e += 32) {
+                const uint32_t at = uint32_t(e) * elem_bytes;
+                const uint32_t src = stage_box + row * 128 + (((at >> 4) ^ (row & 7)) << 4) + (at & 15u);
+                if (elem_bytes == 2) {
+                    uint16_t v;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(src));
+                    reinterpret_cast<uint16_t*>(out)[e] = v;
+                } else {
+                    uint32_t v;
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(src));
+                    reinterpret_cast<uint32_t*>(out)[e] = v;
+                }
+            }
+        }
+    };
+    auto box_free = [&]() {                                  // the box's previous contents have been read
+        if (!p.plain_out && lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
+    };
+    const uint32_t box_row = stage_box + lane * 128;
+    if (p.out_dtype == TKB_DTYPE_FP32) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (col0 + 32 * h >= p.N) return;
+            box_free();
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                st_shared_v4(box_row + ((j ^ (lane & 7)) << 4), r[32 * h + 4 * j], r[32 * h + 4 * j + 1], r[32 * h + 4 * j + 2], r[32 * h + 4 * j + 3]);
+            leave(col0 + 32 * h, 4);
+        }
+        return;
+    }
+    if (p.out_dtype == TKB_DTYPE_FP16) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) r[i] = pack_f16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; i++) r[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+    }
+    box_free();
+#pragma unroll
+    for (int j = 0; j < 8; j++) st_shared_v4(box_row + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+    leave(col0, 2);
 }
 
 // All-gather mode (tensor-parallel GEMM): the A operand is row-sharded over `world` GPUs.  Every rank
@@ -660,6 +746,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                                 mma_f16<CTAS>(acc_h, a_desc + 2 * j, b_desc + 2 * j, idesc_bf16(C::MMA_M, BN), acc);
                             } else if constexpr (KIND == KIND_FP8) {
                                 mma_f8<CTAS>(acc_h, a_desc + 2 * j, b_desc + 2 * j, idesc_fp8(C::MMA_M, BN), acc);
+                            } else if constexpr (KIND == KIND_INT8) {
+                                mma_i8<CTAS>(acc_h, a_desc + 2 * j, b_desc + 2 * j, idesc_int8(C::MMA_M, BN), acc);
                             } else if constexpr (KIND == KIND_MXFP8) {
                                 mma_mxfp8<CTAS>(acc_h, a_desc + 2 * j, b_desc + 2 * j, idesc_mxfp8(C::MMA_M, BN, j), acc, sfa_t, sfb_t);
                             } else {
@@ -709,6 +797,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride) {
             int m_blk, n_blk;
             tile_to_block(tile, tiles_m, tiles_n, tile_group, tile_rot, m_blk, n_blk);
+            float row_scale = 0.f;       // (a row that TMA clips or the plain stores leave out)
+            if constexpr (KIND == KIND_INT8) {
+                const int row = m_blk * C::BM + int(cta_rank) * 128 + quarter * 32 + lane;
+                if (row < p.M) row_scale = __ldg(p.sgA + row);
+            }
+            (void)row_scale;
             const long long t0 = clock64();
             const uint32_t buf = tile_count % C::ACC_BUFS;
             if (!mbar_wait(wc, smem_u32(&bar_tmem_full[buf]), (tile_count / C::ACC_BUFS) & 1u)) { ok = false; break; }
@@ -729,6 +823,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             if (lane == 0 && mh == MH - 1) {                 // the last half is in registers: tensor memory goes back
                 const uint32_t tmem_empty_leader = buf ? tmem_empty_leader1 : tmem_empty_leader0;
                 if constexpr (CTAS == 2) mbar_arrive_cluster(tmem_empty_leader); else mbar_arrive(tmem_empty_leader);
+            }
+            if constexpr (KIND == KIND_INT8) {
+                const int row0 = m_blk * C::BM + int(cta_rank) * 128 + quarter * 32;
+                const int col0 = n_blk * BN + col_base;
+                int8_epilogue(r0, &tmD, p, stage_box, row0, col0, row_scale, lane, d_policy);
+                int8_epilogue(r1, &tmD, p, stage_box, row0, col0 + 64, row_scale, lane, d_policy);
+                continue;
             }
             uint32_t packed[C::COLS_PER_EPI_WARP / 2];
 #pragma unroll
@@ -892,7 +993,8 @@ static cudaError_t launch_t(const GemmArgs& a) {
     cfg.attrs = attr; cfg.numAttrs = 2;
     static const int group_env = getenv("TKB_GEMM_GROUP") ? atoi(getenv("TKB_GEMM_GROUP")) : 0;
     GemmParams p{a.sgA, a.sgB, a.M, a.N, a.K, group_env > 0 ? group_env : 16, 0, a.status, a.prof, api_wait_limit(),
-                 static_cast<uint8_t*>(a.q_codes), static_cast<uint8_t*>(a.q_sc), a.q_sg, a.q_amax, a.q_arith, a.rs_maps, a.rs_rows_per_rank};
+                 static_cast<uint8_t*>(a.q_codes), static_cast<uint8_t*>(a.q_sc), a.q_sg, a.q_amax, a.q_arith, a.rs_maps, a.rs_rows_per_rank,
+                 a.out_dtype, a.plain_out, a.D, a.ldd};
     if (MODE == MODE_RS && a.rs_world > 0) {
         // start with the rows of the next rank, so that the ranks do not all add into the same owner at the same time
         p.group = a.rs_rows_per_rank / C::BM;
@@ -936,6 +1038,7 @@ cudaError_t launch_gemm(const GemmArgs& a) {
         case KIND_MXFP8: return launch_k<KIND_MXFP8>(a);
         case KIND_NVFP4: return launch_k<KIND_NVFP4>(a);
         case KIND_FP8: return launch_k<KIND_FP8>(a);
+        case KIND_INT8: return launch_k<KIND_INT8>(a);
         default: return cudaErrorInvalidValue;
     }
 }

@@ -6,7 +6,8 @@
 
 namespace tkb {
 
-enum GemmKind : int { KIND_BF16 = 0, KIND_MXFP8 = 1, KIND_NVFP4 = 2, KIND_FP8 = 3 };   // FP8: dense e4m3, no scales
+enum GemmKind : int { KIND_BF16 = 0, KIND_MXFP8 = 1, KIND_NVFP4 = 2, KIND_FP8 = 3,   // FP8: dense e4m3, no scales
+                      KIND_INT8 = 4 };   // int8 with int32 accumulation, one fp32 scale per row of A and per row of B
 
 struct QuantWork;
 struct NvQuantArgs;
@@ -76,6 +77,10 @@ struct GemmArgs {
     // MODE_RS: the bf16 tiles are reduce-added into the output of the rank that owns their rows.  rs_maps: `rs_world` tensor maps in
     // DEVICE memory, map i over rank i's output [M / world, N] bf16 (box 64 x 32, 128-byte swizzle, as tmD); rs_rank rotates the tile order
     const CUtensorMap* rs_maps; int rs_rows_per_rank, rs_rank, rs_world;
+    // KIND_INT8: sgA / sgB hold one scale per row; D has out_dtype (TKB_DTYPE_*).  With plain_out D is stored without TMA (its base
+    // or pitch is not a multiple of 16 bytes) from these two
+    int out_dtype, plain_out;
+    void* D; int64_t ldd;
 };
 cudaError_t launch_gemm(const GemmArgs& a);
 int moe_dispatch_ring(int K);     // row slots the MoE dispatch ring gets for hidden size K (needs >= 24)

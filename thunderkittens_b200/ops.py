@@ -162,3 +162,154 @@ def nvfp4_gemm_quant(A, A_sc, A_sg, B, B_sc, B_sg, out_amax, D_codes, D_sc, D_sg
         raise RuntimeError("the fused epilogue offers the 'spec' and 'kernel_ieee' arithmetics")
     L.check(L.lib().tkb_nvfp4_gemm_quant(A.data_ptr(), A_sc.data_ptr(), A_sg.data_ptr(), B.data_ptr(), B_sc.data_ptr(), B_sg.data_ptr(),
                                          out_amax.data_ptr(), D_codes.data_ptr(), D_sc.data_ptr(), D_sg.data_ptr(), M, N, K, _ARITH[arithmetic], _stream()))
+
+
+# ---- 8-bit integer linear layer and the norms around it (no counterpart in the reference) -------------------------------
+# Unlike the entries above these take row-strided tensors (last dimension contiguous), run on the device of their
+# tensors, whichever is current, on that device's current stream, and accept no rows at all.
+
+_HALF = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_FP16}
+_OUT = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_FP16, torch.float32: L.DTYPE_FP32}
+_INT8 = (torch.int8,)
+_FP32 = (torch.float32,)
+
+
+def _bad(t, name: str, dtypes, device, shape) -> None:
+    """Raises the error that _mat or _vec found."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"{name} has dtype {t.dtype}, expected one of {tuple(dtypes)}")
+    if device is not None and t.get_device() != device:
+        raise RuntimeError(f"{name} is on device {t.get_device()}, the first operand on device {device}")
+    if t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple('any' if s is None else s for s in shape)}")
+    raise RuntimeError(f"{name} must have a contiguous last dimension and rows that do not overlap")
+
+
+def _mat(t, name: str, dtypes, device=None, rows=None, cols=None) -> int:
+    """Checks a row-strided matrix and returns its row pitch in elements."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or (device is not None and t.get_device() != device) or t.dim() != 2:
+        _bad(t, name, dtypes, device, (rows, cols))
+    n, k = t.shape
+    if (rows is not None and n != rows) or (cols is not None and k != cols):
+        _bad(t, name, dtypes, device, (rows, cols))
+    if n <= 1:                              # no pitch that anything reads
+        if k > 1 and t.stride(1) != 1:
+            _bad(t, name, dtypes, device, (rows, cols))
+        return k
+    pitch, step = t.stride()
+    if pitch < k or (step != 1 and k > 1):
+        _bad(t, name, dtypes, device, (rows, cols))
+    return pitch
+
+
+def _vec(t, name: str, dtypes, device, n: int) -> int:
+    """Checks a contiguous vector and returns its address."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.get_device() != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        _bad(t, name, dtypes, device, (n,))
+    return t.data_ptr()
+
+
+def _call(device: int, name: str, *args) -> None:
+    """Calls an entry on the current stream of `device`."""
+    f = getattr(L.lib(), name)
+    if torch.cuda.current_device() == device:
+        code = f(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            code = f(*args, torch.cuda.current_stream().cuda_stream)
+    if code:
+        L.check(code)
+
+
+def int8_quantize(A, A_int8, A_sc) -> None:
+    """A (M,K) bf16 or fp16 -> A_int8 (M,K) codes and A_sc (M,) fp32 steps, one per row, in place.
+
+    A_sc = max(amax, 2**-100) / 127 and A_int8 = rint(A * (127 / amax)), the inverse step in fp32 and the product exact; a row that
+    holds an infinity or a NaN gets step NaN and codes 0.  K <= 65536.  As an operand of int8_gemm the rows of A_int8 must begin
+    16 bytes apart: for other K allocate (M, K rounded up to 16) and pass the [:, :K] slice."""
+    lda = _mat(A, "A", _HALF)
+    M, K = A.shape
+    dev = A.get_device()
+    ldc = _mat(A_int8, "A_int8", _INT8, dev, M, K)
+    _call(dev, "tkb_int8_quantize", A.data_ptr(), lda, _HALF[A.dtype], A_int8.data_ptr(), ldc, _vec(A_sc, "A_sc", _FP32, dev, M), M, K)
+
+
+def int8_gemm(A, A_sc, B, B_sc, D, config: str | None = None) -> None:
+    """D (M,N) = A_sc[:, None] * B_sc * (A @ B.T); A (M,K), B (N,K) int8, A_sc (M,), B_sc (N,) fp32, D bf16, fp16 or fp32.
+
+    The sums are exact (K <= 131071).  Rows of A and B begin 16 bytes apart; D may have any row pitch."""
+    lda = _mat(A, "A", _INT8)
+    M, K = A.shape
+    dev = A.get_device()
+    ldb = _mat(B, "B", _INT8, dev, None, K)
+    N = B.shape[0]
+    ldd = _mat(D, "D", _OUT, dev, M, N)
+    L_args = (A.data_ptr(), lda, _vec(A_sc, "A_sc", _FP32, dev, M), B.data_ptr(), ldb, _vec(B_sc, "B_sc", _FP32, dev, N), D.data_ptr(), ldd, _OUT[D.dtype], M, N, K)
+    _call(dev, "tkb_int8_gemm_ex", *L_args, _CONFIG[config])
+
+
+def _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc):
+    """Arguments of the optional outputs of a norm: Y, its pitch, the codes, their pitch, their steps."""
+    y = ldy = q = ldq = sc = 0
+    if Y is not None:
+        ldy = _mat(Y, "Y", (t,), dev, M, K)
+        y = Y.data_ptr()
+    if (Y_int8 is None) != (Y_sc is None):
+        raise RuntimeError("Y_int8 and Y_sc come together")
+    if Y_int8 is not None:
+        ldq = _mat(Y_int8, "Y_int8", _INT8, dev, M, K)
+        q, sc = Y_int8.data_ptr(), _vec(Y_sc, "Y_sc", _FP32, dev, M)
+    return y, ldy, q, ldq, sc
+
+
+def rms_norm(X, W, Y=None, Y_int8=None, Y_sc=None, eps: float = 1e-6) -> None:
+    """y = X * rsqrt(mean(X**2) + eps) * W over the rows of X (M,K) bf16 or fp16, K <= 16384, into Y (M,K) of X's dtype and / or,
+    quantized as by int8_quantize, into Y_int8 (M,K) and Y_sc (M,)."""
+    ldx = _mat(X, "X", _HALF)
+    M, K = X.shape
+    dev, t = X.get_device(), X.dtype
+    w = _vec(W, "W", (t,), dev, K)
+    if Y is None and Y_int8 is None:
+        raise RuntimeError("rms_norm needs Y or Y_int8 and Y_sc")
+    y, ldy, q, ldq, sc = _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc)
+    _call(dev, "tkb_rms_norm", X.data_ptr(), ldx, w, y, ldy, q, ldq, sc, _HALF[t], M, K, eps)
+
+
+def block_norm(H, X, X_out, W_post=None, gate=None, residual_scale: float = 1.0, W_pre=None, Y=None, Y_int8=None, Y_sc=None,
+               eps: float = 1e-6) -> None:
+    """The norm after a block, its gate and residual, and the norm before the next block, over rows (M,K) bf16 or fp16, K <= 16384:
+
+        r = residual_scale * X + gate * norm(H) * W_post  -> X_out        (W_post None: H itself; gate None: 1)
+        y = norm(r) * W_pre                               -> Y and / or Y_int8, Y_sc as in rms_norm (W_pre None: left out)
+
+    gate is (K,), or (G,K) with M a multiple of G: row i uses gate row i // (M // G), that is one gate for each sequence of a
+    batch, or with G = M one for each token.  X_out may be X."""
+    ldh = _mat(H, "H", _HALF)
+    M, K = H.shape
+    dev, t = H.get_device(), H.dtype
+    ldx = _mat(X, "X", (t,), dev, M, K)
+    ldr = _mat(X_out, "X_out", (t,), dev, M, K)
+    w_post = 0 if W_post is None else _vec(W_post, "W_post", (t,), dev, K)
+    w_pre = 0 if W_pre is None else _vec(W_pre, "W_pre", (t,), dev, K)
+    g = ldg = 0
+    per = 1
+    if gate is not None:
+        if isinstance(gate, torch.Tensor) and gate.dim() == 1:
+            g, ldg, per = _vec(gate, "gate", (t,), dev, K), K, max(M, 1)
+        else:
+            ldg = _mat(gate, "gate", (t,), dev, None, K)
+            G = gate.shape[0]
+            if (M % G if G else M) or (M and M < G):
+                raise RuntimeError(f"gate has {G} rows, of which {M} rows of H are no multiple")
+            g, per = gate.data_ptr(), max(M // G, 1) if G else 1
+    if W_pre is None and (Y is not None or Y_int8 is not None):
+        raise RuntimeError("Y and Y_int8 need W_pre")
+    if W_pre is not None and Y is None and Y_int8 is None:
+        raise RuntimeError("W_pre needs Y or Y_int8 and Y_sc")
+    y, ldy, q, ldq, sc = _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc)
+    _call(dev, "tkb_block_norm", H.data_ptr(), ldh, X.data_ptr(), ldx, X_out.data_ptr(), ldr, w_post, g, ldg, per, residual_scale,
+          w_pre, y, ldy, q, ldq, sc, _HALF[t], M, K, eps)
