@@ -347,6 +347,16 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
         return api_fail(TKB_ERR_BAD_ALIGNMENT, "int8_gemm: scales and D must be aligned to their element type");
     DeviceCtx* c;
     if (int e = get_ctx(&c)) return e;
+    if (M <= kInt8SkinnyMaxM && config == TKB_GEMM_DEFAULT) {
+        SkinnyArgs a;
+        memset(&a, 0, sizeof(a));
+        if (int e = make_operand_map(&a.tmW, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, ldb, int8_skinny_slab_rows(M, N, K, c->sm_count))) return e;
+        if (int e = make_operand_map(&a.tmX, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, lda, int8_skinny_padded_rows(M))) return e;
+        a.a_sc = A_sc; a.b_sc = B_sc; a.D = D; a.ldd = ldd; a.M = M; a.N = N; a.K = K; a.out_dtype = dtype;
+        a.status = c->status; a.sm_count = c->sm_count; a.stream = static_cast<cudaStream_t>(stream);
+        TKB_CUDA(launch_int8_skinny(a));
+        return TKB_OK;
+    }
     GemmArgs g;
     memset(&g, 0, sizeof(g));
     g.kind = KIND_INT8;

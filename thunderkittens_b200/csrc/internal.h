@@ -102,4 +102,17 @@ struct DecodeArgs {
 cudaError_t launch_decode(const DecodeArgs& a);
 int decode_padded_rows(int M);
 
+// int8_skinny.cu
+constexpr int kInt8SkinnyMaxM = 128;
+struct SkinnyArgs {
+    CUtensorMap tmW, tmX;       // boxes of 128 bytes of K x int8_skinny_slab_rows() weight rows / int8_skinny_padded_rows() tokens, 128-byte swizzle
+    const float* a_sc; const float* b_sc;
+    void* D; int64_t ldd;
+    int M, N, K, out_dtype;
+    int* status; int sm_count; cudaStream_t stream;
+};
+cudaError_t launch_int8_skinny(const SkinnyArgs& a);
+int int8_skinny_padded_rows(int M);
+int int8_skinny_slab_rows(int M, int N, int K, int sm_count);
+
 } // namespace tkb
