@@ -189,38 +189,50 @@ def _bad(t, name: str, dtypes, device, shape) -> None:
     raise RuntimeError(f"{name} must have a contiguous last dimension and rows that do not overlap")
 
 
-def _mat(t, name: str, dtypes, device=None, rows=None, cols=None) -> int:
-    """Checks a row-strided matrix and returns its row pitch in elements."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or (device is not None and t.get_device() != device) or t.dim() != 2:
-        _bad(t, name, dtypes, device, (rows, cols))
+# The checks below run before every launch and count where a call takes microseconds: each asks a tensor once for each property.
+
+def _first(t, name: str, dtypes):
+    """Checks the matrix that fixes a call's rows, columns and device: (rows, columns, device, row pitch in elements)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or t.dim() != 2:
+        _bad(t, name, dtypes, None, (None, None))
     n, k = t.shape
-    if (rows is not None and n != rows) or (cols is not None and k != cols):
-        _bad(t, name, dtypes, device, (rows, cols))
-    if n <= 1:                              # no pitch that anything reads
-        if k > 1 and t.stride(1) != 1:
-            _bad(t, name, dtypes, device, (rows, cols))
-        return k
     pitch, step = t.stride()
+    if n <= 1:                              # no pitch that anything reads
+        pitch = k
     if pitch < k or (step != 1 and k > 1):
-        _bad(t, name, dtypes, device, (rows, cols))
-    return pitch
+        _bad(t, name, dtypes, None, (n, k))
+    return n, k, t.get_device(), pitch
 
 
-def _vec(t, name: str, dtypes, device, n: int) -> int:
+def _mat(t, name: str, dtypes, device: int, n: int, k: int) -> int:
+    """Checks a row-strided [n, k] matrix and returns its row pitch in elements."""
+    if isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype in dtypes and t.shape == (n, k):
+        pitch, step = t.stride()
+        if n <= 1:
+            pitch = k
+        if pitch >= k and (step == 1 or k <= 1):
+            return pitch
+    _bad(t, name, dtypes, device, (n, k))
+
+
+def _vec(t, name: str, dtypes, device: int, n: int) -> int:
     """Checks a contiguous vector and returns its address."""
-    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.get_device() != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dtype not in dtypes or t.shape != (n,) or not t.is_contiguous():
         _bad(t, name, dtypes, device, (n,))
     return t.data_ptr()
 
 
-def _call(device: int, name: str, *args) -> None:
-    """Calls an entry on the current stream of `device`."""
-    f = getattr(L.lib(), name)
-    if torch.cuda.current_device() == device:
-        code = f(*args, torch.cuda.current_stream().cuda_stream)
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _call(device: int, entry, *args) -> None:
+    """Calls an entry on the current stream of `device` (its handle alone: torch.cuda.current_stream() builds a Stream object
+    around it, 3 us; a tensor of the call is on the GPU, so CUDA is initialised)."""
+    if _current_device() == device:
+        code = entry(*args, _current_stream(device))
     else:
         with torch.cuda.device(device):
-            code = f(*args, torch.cuda.current_stream().cuda_stream)
+            code = entry(*args, _current_stream(device))
     if code:
         L.check(code)
 
@@ -231,25 +243,22 @@ def int8_quantize(A, A_int8, A_sc) -> None:
     A_sc = max(amax, 2**-100) / 127 and A_int8 = rint(A * (127 / amax)), the inverse step in fp32 and the product exact; a row that
     holds an infinity or a NaN gets step NaN and codes 0.  K <= 65536.  As an operand of int8_gemm the rows of A_int8 must begin
     16 bytes apart: for other K allocate (M, K rounded up to 16) and pass the [:, :K] slice."""
-    lda = _mat(A, "A", _HALF)
-    M, K = A.shape
-    dev = A.get_device()
+    M, K, dev, lda = _first(A, "A", _HALF)
     ldc = _mat(A_int8, "A_int8", _INT8, dev, M, K)
-    _call(dev, "tkb_int8_quantize", A.data_ptr(), lda, _HALF[A.dtype], A_int8.data_ptr(), ldc, _vec(A_sc, "A_sc", _FP32, dev, M), M, K)
+    _call(dev, L.lib().tkb_int8_quantize, A.data_ptr(), lda, _HALF[A.dtype], A_int8.data_ptr(), ldc, _vec(A_sc, "A_sc", _FP32, dev, M), M, K)
 
 
 def int8_gemm(A, A_sc, B, B_sc, D, config: str | None = None) -> None:
     """D (M,N) = A_sc[:, None] * B_sc * (A @ B.T); A (M,K), B (N,K) int8, A_sc (M,), B_sc (N,) fp32, D bf16, fp16 or fp32.
 
     The sums are exact (K <= 131071).  Rows of A and B begin 16 bytes apart; D may have any row pitch."""
-    lda = _mat(A, "A", _INT8)
-    M, K = A.shape
-    dev = A.get_device()
-    ldb = _mat(B, "B", _INT8, dev, None, K)
-    N = B.shape[0]
+    M, K, dev, lda = _first(A, "A", _INT8)
+    N, KB, devB, ldb = _first(B, "B", _INT8)
+    if KB != K or devB != dev:
+        _bad(B, "B", _INT8, dev, (None, K))
     ldd = _mat(D, "D", _OUT, dev, M, N)
-    L_args = (A.data_ptr(), lda, _vec(A_sc, "A_sc", _FP32, dev, M), B.data_ptr(), ldb, _vec(B_sc, "B_sc", _FP32, dev, N), D.data_ptr(), ldd, _OUT[D.dtype], M, N, K)
-    _call(dev, "tkb_int8_gemm_ex", *L_args, _CONFIG[config])
+    _call(dev, L.lib().tkb_int8_gemm_ex, A.data_ptr(), lda, _vec(A_sc, "A_sc", _FP32, dev, M), B.data_ptr(), ldb, _vec(B_sc, "B_sc", _FP32, dev, N),
+          D.data_ptr(), ldd, _OUT[D.dtype], M, N, K, _CONFIG[config])
 
 
 def _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc):
@@ -269,14 +278,13 @@ def _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc):
 def rms_norm(X, W, Y=None, Y_int8=None, Y_sc=None, eps: float = 1e-6) -> None:
     """y = X * rsqrt(mean(X**2) + eps) * W over the rows of X (M,K) bf16 or fp16, K <= 16384, into Y (M,K) of X's dtype and / or,
     quantized as by int8_quantize, into Y_int8 (M,K) and Y_sc (M,)."""
-    ldx = _mat(X, "X", _HALF)
-    M, K = X.shape
-    dev, t = X.get_device(), X.dtype
+    M, K, dev, ldx = _first(X, "X", _HALF)
+    t = X.dtype
     w = _vec(W, "W", (t,), dev, K)
     if Y is None and Y_int8 is None:
         raise RuntimeError("rms_norm needs Y or Y_int8 and Y_sc")
     y, ldy, q, ldq, sc = _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc)
-    _call(dev, "tkb_rms_norm", X.data_ptr(), ldx, w, y, ldy, q, ldq, sc, _HALF[t], M, K, eps)
+    _call(dev, L.lib().tkb_rms_norm, X.data_ptr(), ldx, w, y, ldy, q, ldq, sc, _HALF[t], M, K, eps)
 
 
 def block_norm(H, X, X_out, W_post=None, gate=None, residual_scale: float = 1.0, W_pre=None, Y=None, Y_int8=None, Y_sc=None,
@@ -288,9 +296,8 @@ def block_norm(H, X, X_out, W_post=None, gate=None, residual_scale: float = 1.0,
 
     gate is (K,), or (G,K) with M a multiple of G: row i uses gate row i // (M // G), that is one gate for each sequence of a
     batch, or with G = M one for each token.  X_out may be X."""
-    ldh = _mat(H, "H", _HALF)
-    M, K = H.shape
-    dev, t = H.get_device(), H.dtype
+    M, K, dev, ldh = _first(H, "H", _HALF)
+    t = H.dtype
     ldx = _mat(X, "X", (t,), dev, M, K)
     ldr = _mat(X_out, "X_out", (t,), dev, M, K)
     w_post = 0 if W_post is None else _vec(W_post, "W_post", (t,), dev, K)
@@ -301,8 +308,9 @@ def block_norm(H, X, X_out, W_post=None, gate=None, residual_scale: float = 1.0,
         if isinstance(gate, torch.Tensor) and gate.dim() == 1:
             g, ldg, per = _vec(gate, "gate", (t,), dev, K), K, max(M, 1)
         else:
-            ldg = _mat(gate, "gate", (t,), dev, None, K)
-            G = gate.shape[0]
+            G, KG, devG, ldg = _first(gate, "gate", (t,))
+            if KG != K or devG != dev:
+                _bad(gate, "gate", (t,), dev, (None, K))
             if (M % G if G else M) or (M and M < G):
                 raise RuntimeError(f"gate has {G} rows, of which {M} rows of H are no multiple")
             g, per = gate.data_ptr(), max(M // G, 1) if G else 1
@@ -311,5 +319,5 @@ def block_norm(H, X, X_out, W_post=None, gate=None, residual_scale: float = 1.0,
     if W_pre is not None and Y is None and Y_int8 is None:
         raise RuntimeError("W_pre needs Y or Y_int8 and Y_sc")
     y, ldy, q, ldq, sc = _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc)
-    _call(dev, "tkb_block_norm", H.data_ptr(), ldh, X.data_ptr(), ldx, X_out.data_ptr(), ldr, w_post, g, ldg, per, residual_scale,
+    _call(dev, L.lib().tkb_block_norm, H.data_ptr(), ldh, X.data_ptr(), ldx, X_out.data_ptr(), ldr, w_post, g, ldg, per, residual_scale,
           w_pre, y, ldy, q, ldq, sc, _HALF[t], M, K, eps)
