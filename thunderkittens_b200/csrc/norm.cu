@@ -250,9 +250,11 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
                 uint32_t h[P];
                 S::take(slot_h, K, shift, h);
                 if (next < p.M) fetch(next, next_shift);
+#pragma unroll
+                for (int i = 0; i < P; i++) v[i] = up2<T>(h[i]);
                 if (p.w_post) {
 #pragma unroll
-                    for (int i = 0; i < P; i++) sum = fma2(up2<T>(h[i]), up2<T>(h[i]), sum);
+                    for (int i = 0; i < P; i++) sum = fma2(v[i], v[i], sum);
                     float s1;
                     split(sum, s, s1);
                     s += s1;
@@ -264,8 +266,6 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
 #pragma unroll
                 for (int g = 0; g < V; g++) {
                     uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v[4 * g + i] = up2<T>(h[4 * g + i]);
                     if (p.w_post) {
                         S::peek(static_cast<const uint16_t*>(p.w_post), K, shift, g, w);
 #pragma unroll
@@ -295,8 +295,8 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
                     S::peek(static_cast<const uint16_t*>(p.w_pre), K, shift, g, w);
 #pragma unroll
                     for (int i = 4 * g; i < 4 * g + 4; i++) {
-                        if (MODE == ROWS_BLOCK) {
-                            // elements outside the row are made zeros, whatever the scales, gates and weights that they met
+                        if (MODE == ROWS_BLOCK && W != 8) {
+                            // outside the row h and x are zeros, but the gates and weights that they met may be no numbers
                             const int e0 = S::at(2 * i, shift), e1 = S::at(2 * i + 1, shift);
                             float lo, hi;
                             split(v[i], lo, hi);
@@ -396,6 +396,7 @@ static int rows_call(const char* what, RowsParams p, int mode, int dtype, void* 
     const int max_k = mode == ROWS_QUANT ? kQuantMaxK : kNormMaxK;
     if (p.K > max_k) return api_fail(TKB_ERR_INVALID_ARG, "%s: K=%d is above %d, the longest row that one CTA holds", what, p.K, max_k);
     if ((p.codes == nullptr) != (p.sc == nullptr) && p.M > 0) return api_fail(TKB_ERR_INVALID_ARG, "%s: int8 codes and their scales come together", what);
+    if (mode == ROWS_BLOCK && !(p.residual_scale >= -1e30f && p.residual_scale <= 1e30f)) return api_fail(TKB_ERR_INVALID_ARG, "%s: residual_scale must be a number", what);
     if (mode != ROWS_QUANT && !(p.eps >= 0.0f && p.eps < 1e30f)) return api_fail(TKB_ERR_INVALID_ARG, "%s: eps must be a number >= 0", what);
     if (p.M > 0) {
         if (!p.x) return api_fail(TKB_ERR_INVALID_ARG, "%s: null input", what);
