@@ -174,6 +174,18 @@ def test_gemm_repeats_bit_for_bit(cuda, lib):
         assert torch.equal(D[0], D[1]) and torch.equal(D[0], D[2])
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 96, 2048), (5, 2048, 1024), (33, 77, 2000), (65, 77, 2000), (128, 1000, 4096)])
+def test_gemm_split_over_a_cluster_many_times(cuda, lib, M, N, K):
+    """K split over the CTAs of a cluster, back to back: every launch exchanges its sums before the next one begins."""
+    a, a_sc, b, b_sc = _operands(M, N, K, cuda, seed=8)
+    D = [torch.full((M, N), float("nan"), device=cuda) for _ in range(40)]
+    for _ in range(10):
+        for d in D:
+            _ops().int8_gemm(a, a_sc, b, b_sc, d)
+    _check_gemm(D[0], a, a_sc, b, b_sc)
+    assert all(torch.equal(d, D[0]) for d in D[1:])
+
+
 @pytest.mark.parametrize("N", [60000, 60001])
 def test_gemm_output_past_32_bit_offsets(cuda, lib, N):
     M, K = 40000, 16

@@ -56,6 +56,11 @@ __device__ __forceinline__ void tmem_ld_32x16_i(uint32_t taddr, uint32_t* r) {
         : "memory");
 }
 
+// Cluster barrier of warps whose lanes may come out of a wait one after the other: the forms without .aligned, and the lanes
+// together first.
+__device__ __forceinline__ void split_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void split_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); __syncwarp(); }
+
 __device__ __forceinline__ void store_out(const SkinnyParams& p, int m, int n, int sum, float a_sc, float b_sc) {
     const float v = __int2float_rn(sum) * a_sc * b_sc;
     const int64_t at = int64_t(m) * p.ldd + n;
@@ -130,7 +135,7 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         }
         __syncwarp();
-        if (split > 1) cluster_arrive();    // (1): the epilogue warps arrive when this CTA's MMAs are done
+        if (split > 1) split_arrive();      // (1): the epilogue warps arrive when this CTA's MMAs are done
         if (leader) {
             for (int s = 0; s < nst && ok; s++) {                   // stage releases of the MMA thread may still be in flight
                 ok = mbar_wait(wc, smem_u32(&bar_empty[stage]), phase ^ 1);
@@ -139,7 +144,7 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             if (!ok) drain_ring(bar_full, nst, issued, p.wait_limit);
         }
         __syncwarp();
-        if (split > 1) { cluster_wait(); cluster_sync(); }
+        if (split > 1) { split_wait(); split_arrive(); split_wait(); }
     } else if (warp == 1) {
         if (elect_one()) {
             uint32_t stage = 0, phase = 0, seg = 0;
@@ -163,7 +168,7 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             }
         }
         __syncwarp();
-        if (split > 1) { cluster_sync(); cluster_sync(); }
+        if (split > 1) { split_arrive(); split_wait(); split_arrive(); split_wait(); }
     } else {
         const int quarter = warp & 3;
         const int n_local = quarter * 32 + lane;
@@ -175,7 +180,8 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 const int n = slab * p.rows + n_local;
                 const bool mine = n_local < p.rows && n < p.N;
                 const float b_sc = mine ? __ldg(p.b_sc + n) : 0.f;
-                if (!mbar_wait(wc, smem_u32(&bar_acc_full[buf]), (seg >> 1) & 1u)) break;
+                const bool full = mbar_wait(wc, smem_u32(&bar_acc_full[buf]), (seg >> 1) & 1u);
+                if (!__all_sync(0xffffffffu, full)) break;          // (lanes together: the loads below are the warp's)
                 tc_fence_after();
 #pragma unroll
                 for (int c0 = 0; c0 < NB; c0 += C::CHUNK) {
@@ -200,9 +206,10 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             const int n = unit * p.rows + n_local;
             const bool mine = n_local < p.rows && n < p.N;
             const float b_sc = mine ? __ldg(p.b_sc + n) : 0.f;
-            const bool ok = mbar_wait(wc, smem_u32(&bar_acc_full[0]), 0);
+            const bool ok = __all_sync(0xffffffffu, mbar_wait(wc, smem_u32(&bar_acc_full[0]), 0));
             tc_fence_after();
-            cluster_sync();                                         // every CTA's MMAs are done: the rings may be written over
+            split_arrive();                                         // (1)
+            split_wait();                                           // every CTA's MMAs are done: the rings may be written over
             if (ok) {
 #pragma unroll
                 for (int c0 = 0; c0 < NB; c0 += C::CHUNK) {
@@ -224,7 +231,8 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 }
             }
             tc_fence_before();
-            cluster_sync();                                         // the partial sums sent above are where they belong
+            split_arrive();                                         // (2)
+            split_wait();                                           // the partial sums sent above are where they belong
             if (ok && mine) {
                 for (int g = rank; 4 * g < p.M; g += split) {
                     const uint32_t src = sRecv + uint32_t((g - rank) * 128 + n_local) * 16;
