@@ -1,15 +1,16 @@
 // Row kernels in front of the 8-bit integer GEMM: per-token int8 quantization and the norms around a block.
 //
-// A CTA holds a row of K elements in registers, so every operator here is ONE pass over its data:
+// A group of threads holds a row of K elements in registers, so every operator here is ONE pass over its data:
 //   ROWS_QUANT  codes = rint(x * fl32(127 / amax)), sc = fl32(amax / 127), amax = max(max |x|, 2^-100)
 //   ROWS_NORM   y = x * w_pre * rsqrt(mean(x^2) + eps)
 //   ROWS_BLOCK  p = h * rsqrt(mean(h^2) + eps) * w_post (or h); r = residual_scale * x + gate * p; y from r as above
 // y leaves as 16-bit values, or quantized like ROWS_QUANT, or both.  All of it is arithmetic in fp32: r and y are rounded
 // to 16 bits only where they are stored, and y comes from the unrounded r, the codes from the unrounded y.
 //
-// Bound by HBM.  CTAs are persistent; while one works on a row in its registers, its next row is on the way to shared memory, so
+// Bound by HBM.  CTAs are persistent; while a group works on a row in its registers, its next row is on the way to shared memory, so
 // that loads are in flight all the time and cost no registers.  The largest |y| is rsqrt(..) times the largest |x * w_pre| (rounding
-// is monotonic), so the sum of squares and the maximum share one reduction over the CTA.
+// is monotonic), so the sum of squares and the maximum share one reduction.  Next after HBM comes the issue of instructions: fp32
+// arithmetic on register pairs, and, where a CTA has many rows, weights in shared memory as fp32, for all groups of the CTA.
 //
 // No counterpart in the reference, whose quantizers are block-scaled; the operators stand next to those (quantize.cu).
 #include <atomic>
@@ -23,6 +24,15 @@ int api_fail(int code, const char* fmt, ...);          // api.cu
 int api_device(int* sm_count, int** status);
 
 enum RowsMode : int { ROWS_QUANT = 0, ROWS_NORM = 1, ROWS_BLOCK = 2 };
+// How a thread's elements lie in memory:
+//   ROWS_WHOLE    groups of 8 in 16-byte accesses: K, the pitches and the bases allow it
+//   ROWS_SHIFTED  the same for rows that begin anywhere, but all of the call's row tensors alike within 16 bytes: groups begin `shift`
+//                 elements before the row, its first and last group are partial
+//   ROWS_SINGLE   single elements, where the tensors begin differently
+enum RowsKind : int { ROWS_WHOLE = 0, ROWS_SHIFTED = 1, ROWS_SINGLE = 2 };
+// How rows share a CTA: one row each (everything that depends on the row is uniform over the CTA); a row for each warp (no barriers);
+// several groups of warps with a row each, which also share weights in shared memory
+enum RowsLayout : int { ROWS_ONE = 0, ROWS_WARPS = 1, ROWS_STAGED = 2 };
 constexpr int kNormMaxK = 16384, kQuantMaxK = 65536;
 
 struct RowsParams {
@@ -58,89 +68,117 @@ template <typename T> __device__ __forceinline__ uint32_t down2(F2 a) { float lo
 // max(|m|, |a|, |b|); a NaN stays one
 __device__ __forceinline__ float max_abs3(float m, float a, float b) { float d; asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(a), "f"(b)); return d; }
 
-// The elements of a row that a thread holds, and how it reaches them in memory, W at a time:
-//   W = 8  groups of 8 in 16-byte accesses: K, the pitches and the bases allow it
-//   W = 2  pairs in 4-byte accesses, for odd K or pitches: in a row that begins in the middle of a word the pairs begin one
-//          element earlier (`shift` = 1) in all of the call's row tensors alike
-//   W = 1  single elements, where the tensors begin differently
-template <int V, int W>
+// The 8 V elements of a row that a thread holds, in 4 V pairs
+template <int V, int KIND>
 struct Slots {
-    static constexpr int E = 8 * V;
-    static __device__ __forceinline__ int at(int j, int shift) { return (int(threadIdx.x) + (j / W) * int(blockDim.x)) * W + j % W - (W == 2 ? shift : 0); }
-    // a row tensor's elements into the thread's own words of shared memory, asynchronously where the access is 4 bytes or more
+    static constexpr int P = 4 * V;
+    static __device__ __forceinline__ int at(int j, int shift) {
+        if (KIND == ROWS_SINGLE) return int(threadIdx.x) + j * int(blockDim.x);
+        return (int(threadIdx.x) + (j >> 3) * int(blockDim.x)) * 8 + (j & 7) - (KIND == ROWS_SHIFTED ? shift : 0);
+    }
+    // address of words 4 g .. 4 g + 3 of the thread in a slot
+    static __device__ __forceinline__ uint32_t word(uint32_t slot, int g) { return slot + (g * blockDim.x + threadIdx.x) * 16; }
+
+    // a row into the thread's own words of shared memory, asynchronously where a group is whole
     static __device__ __forceinline__ void fetch(const uint16_t* row, int K, int shift, uint32_t slot) {
-        if constexpr (W == 8) {
 #pragma unroll
-            for (int i = 0; i < V; i++)
-                if (at(8 * i, 0) < K)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + (i * blockDim.x + threadIdx.x) * 16), "l"(row + at(8 * i, 0)) : "memory");
-        } else {
-#pragma unroll
-            for (int i = 0; i < E / 2; i++) {
-                const int e0 = at(2 * i, shift), e1 = at(2 * i + 1, shift);
-                const uint32_t dst = slot + (i * blockDim.x + threadIdx.x) * 4;
-                if constexpr (W == 2) {
-                    if (e0 >= 0 && e1 < K) asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(row + e0) : "memory");
-                    if (e1 == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(uint32_t(row[0]) << 16) : "memory");
-                    if (e0 == K - 1) asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(uint32_t(row[e0])) : "memory");
-                } else if (e0 < K) {
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(row[e0] | (e1 < K ? uint32_t(row[e1]) << 16 : 0u)) : "memory");
-                }
+        for (int g = 0; g < V; g++) {
+            const int e = at(8 * g, shift);
+            if (KIND == ROWS_WHOLE ? e < K : (KIND == ROWS_SHIFTED && e >= 0 && e + 8 <= K)) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(word(slot, g)), "l"(row + e) : "memory");
+            } else if (KIND != ROWS_WHOLE && e < K) {
+                uint32_t w[4];
+                gather(row, K, shift, g, w);
+                st_shared_v4(word(slot, g), w[0], w[1], w[2], w[3]);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    static __device__ __forceinline__ void take(uint32_t slot, int K, int shift, uint32_t (&w)[E / 2]) {
-        if constexpr (W == 8) {
+    // the elements of group g that lie in the row, one by one; zeros for the others
+    static __device__ __forceinline__ void gather(const uint16_t* row, int K, int shift, int g, uint32_t (&w)[4]) {
+        if (KIND == ROWS_SHIFTED && at(8 * g, shift) >= 0 && at(8 * g, shift) + 8 <= K) {
+            const uint16_t* q = row + at(8 * g, shift);
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                w[4 * i] = w[4 * i + 1] = w[4 * i + 2] = w[4 * i + 3] = 0;
-                if (at(8 * i, 0) < K)
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3])
-                                 : "r"(slot + (i * blockDim.x + threadIdx.x) * 16)
-                                 : "memory");
-            }
-        } else {
+            for (int i = 0; i < 4; i++) w[i] = q[2 * i] | uint32_t(q[2 * i + 1]) << 16;
+            return;
+        }
 #pragma unroll
-            for (int i = 0; i < E / 2; i++) {
-                w[i] = 0;
-                if (at(2 * i, shift) < K) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(slot + (i * blockDim.x + threadIdx.x) * 4) : "memory");
+        for (int i = 0; i < 4; i++) {
+            const int e0 = at(8 * g + 2 * i, shift), e1 = at(8 * g + 2 * i + 1, shift);
+            w[i] = e0 >= 0 && e0 < K ? row[e0] : 0u;
+            if (e1 >= 0 && e1 < K) w[i] |= uint32_t(row[e1]) << 16;
+        }
+    }
+    static __device__ __forceinline__ void take(uint32_t slot, int K, int shift, uint32_t (&w)[P]) {
+#pragma unroll
+        for (int g = 0; g < V; g++) {
+            w[4 * g] = w[4 * g + 1] = w[4 * g + 2] = w[4 * g + 3] = 0;
+            if (at(8 * g, shift) < K)
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[4 * g]), "=r"(w[4 * g + 1]), "=r"(w[4 * g + 2]), "=r"(w[4 * g + 3])
+                             : "r"(word(slot, g))
+                             : "memory");
+        }
+    }
+    static __device__ __forceinline__ void store(uint16_t* row, int K, int shift, const uint32_t (&w)[P]) {
+#pragma unroll
+        for (int g = 0; g < V; g++) {
+            const int e = at(8 * g, shift);
+            if (KIND == ROWS_WHOLE ? e < K : (KIND == ROWS_SHIFTED && e >= 0 && e + 8 <= K)) {
+                *reinterpret_cast<uint4*>(row + e) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+            } else if (KIND != ROWS_WHOLE && e < K) {
+#pragma unroll
+                for (int i = 4 * g; i < 4 * g + 4; i++) {
+                    const int e0 = at(2 * i, shift), e1 = at(2 * i + 1, shift);
+                    if (e0 >= 0 && e0 < K) row[e0] = uint16_t(w[i]);
+                    if (e1 >= 0 && e1 < K) row[e1] = uint16_t(w[i] >> 16);
+                }
             }
         }
     }
-    // group g (8 elements: 4 words) of a tensor that every row reads (weights, gates): from L1, and again where it is needed
-    // again, rather than kept in registers
-    static __device__ __forceinline__ void peek(const uint16_t* row, int K, int shift, int g, uint32_t (&w)[4]) {
-        if constexpr (W == 8) {
-            w[0] = w[1] = w[2] = w[3] = 0;
-            if (at(8 * g, 0) < K)
-                asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(row + at(8 * g, 0)));
+    // group g of a vector that every row meets (weights, gates), from L1, and again where it is needed again
+    template <typename T>
+    static __device__ __forceinline__ void peek(const void* vec, int K, int shift, int g, F2 (&w)[4]) {
+        uint32_t b[4] = {0u, 0u, 0u, 0u};
+        const uint16_t* v = static_cast<const uint16_t*>(vec);
+        if constexpr (KIND == ROWS_WHOLE) {
+            if (at(8 * g, 0) < K) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "l"(v + at(8 * g, 0)));
         } else {
-            // outside the row any element will do: it meets a zero
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int e0 = min(max(at(8 * g + 2 * i, shift), 0), K - 1), e1 = min(at(8 * g + 2 * i + 1, shift), K - 1);
-                w[i] = __ldg(row + e0) | uint32_t(__ldg(row + e1)) << 16;
-            }
+            gather(v, K, shift, g, b);
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = up2<T>(b[i]);
     }
-    static __device__ __forceinline__ void store(uint16_t* row, int K, int shift, const uint32_t (&w)[E / 2]) {
-        if constexpr (W == 8) {
-#pragma unroll
-            for (int i = 0; i < V; i++)
-                if (at(8 * i, 0) < K) *reinterpret_cast<uint4*>(row + at(8 * i, 0)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    // The same from shared memory as fp32.  Layouts without bank conflicts: WHOLE two halves, of the first and last 4 of every group
+    // (16-byte accesses); SHIFTED one word of padding for every 8, with 8 zeros before and behind the row.
+    static __device__ __forceinline__ int staged_words(int K) { return KIND == ROWS_WHOLE ? K : (KIND == ROWS_SHIFTED ? (K + 24) / 8 * 9 : K); }
+    static __device__ __forceinline__ int staged_at(int e, int K) {
+        return KIND == ROWS_WHOLE ? ((e >> 2) & 1) * (K / 2) + (e >> 3) * 4 + (e & 3) : (KIND == ROWS_SHIFTED ? e + 8 + ((e + 8) >> 3) : e);
+    }
+    static __device__ __forceinline__ void staged(const float* vec, int K, int shift, int g, F2 (&w)[4]) {
+        if constexpr (KIND == ROWS_WHOLE) {
+            const int e = at(8 * g, 0);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+            if (e < K) {
+                a = *reinterpret_cast<const float4*>(vec + e / 2);
+                b = *reinterpret_cast<const float4*>(vec + K / 2 + e / 2);
+            }
+            w[0] = f2(a.x, a.y); w[1] = f2(a.z, a.w); w[2] = f2(b.x, b.y); w[3] = f2(b.z, b.w);
         } else {
+            if constexpr (KIND == ROWS_SHIFTED) {
+                // staged_at(8 c - shift + j) = 9 (c + 1) - shift + j - (j < shift), c the group's number: one address for all but `shift`
+                const float* q = vec + 9 * (int(threadIdx.x) + g * int(blockDim.x) + 1) - shift;
+                const bool in = at(8 * g, shift) < K;
 #pragma unroll
-            for (int i = 0; i < E / 2; i++) {
-                const int e0 = at(2 * i, shift), e1 = at(2 * i + 1, shift);
-                if constexpr (W == 2) {
-                    if (e0 >= 0 && e1 < K) *reinterpret_cast<uint32_t*>(row + e0) = w[i];
-                    if (e1 == 0) row[0] = uint16_t(w[i] >> 16);
-                    if (e0 == K - 1) row[e0] = uint16_t(w[i]);
-                } else {
-                    if (e0 < K) row[e0] = uint16_t(w[i]);
-                    if (e1 < K) row[e1] = uint16_t(w[i] >> 16);
+                for (int i = 0; i < 4; i++) {
+                    const int j0 = 2 * i - (2 * i < shift), j1 = 2 * i + 1 - (2 * i + 1 < shift);
+                    w[i] = in ? f2(q[j0], q[j1]) : f2(0.f, 0.f);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e0 = at(8 * g + 2 * i, shift), e1 = at(8 * g + 2 * i + 1, shift);
+                    w[i] = f2(e0 < K ? vec[e0] : 0.f, e1 < K ? vec[e1] : 0.f);
                 }
             }
         }
@@ -157,16 +195,18 @@ __device__ __forceinline__ float warp_max_abs(float m) {
     asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(m));
     return d;
 }
-// Sum of s and maximum of m >= 0 (or NaN) over the CTA, the same values in every thread.  `part` is shared memory that no thread
-// can still be reading: the CTA has passed a barrier since it last used it.
-template <bool SUM, bool MAX>
-__device__ __forceinline__ void cta_reduce(float& s, float& m, float2* part) {
+// Sum of s and maximum of m >= 0 (or NaN) over the threads of a row (threadIdx.y), the same values in each.  `part` is shared memory
+// that none of them can still be reading: they have passed a barrier since they last used it.
+template <bool SUM, bool MAX, int LAYOUT>
+__device__ __forceinline__ void row_reduce(float& s, float& m, float2* part) {
     const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
     if (SUM) s = warp_sum(s);
     if (MAX) m = warp_max_abs(m);
-    if (nw == 1) return;
+    if (LAYOUT == ROWS_WARPS || nw == 1) return;
     if (lane == 0) part[threadIdx.x >> 5] = make_float2(s, m);
-    __syncthreads();
+    // (a barrier chosen at run time takes all 16 of the CTA, so that no more than 4 CTAs fit an SM: only where rows share a CTA)
+    if (LAYOUT == ROWS_STAGED) asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.y), "r"(blockDim.x) : "memory");
+    else __syncthreads();
     const float2 q = lane < nw ? part[lane] : make_float2(0.f, 0.f);
     if (SUM) s = warp_sum(q.x);
     if (MAX) m = warp_max_abs(q.y);
@@ -176,9 +216,9 @@ __device__ __forceinline__ void cta_reduce(float& s, float& m, float2* part) {
 // the halves-to-even rounding of the exact product value * inv: the fused multiply-add rounds once, to the integer grid that adding
 // 1.5 * 2^23 leaves, and the low byte is the two's complement of the code.  |value| <= m, hence |code| <= 127.  A row that holds an
 // infinity or a NaN has step NaN and codes 0: its products are NaN, and no garbage is taken for a number.
-template <int V, int W, typename F>
+template <int V, int KIND, typename F>
 __device__ __forceinline__ void quantize_row(const RowsParams& p, int row, int shift, float m, F value) {
-    using S = Slots<V, W>;
+    using S = Slots<V, KIND>;
     const bool fine = m < __uint_as_float(0x7f800000u);
     const float amax = fmaxf(m, 0x1p-100f);
     const float inv = __fdiv_rn(127.0f, amax);
@@ -191,48 +231,103 @@ __device__ __forceinline__ void quantize_row(const RowsParams& p, int row, int s
         split(fma2(value(i), inv2, grid), lo, hi);
         return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x0040);
     };
-    if constexpr (W == 8) {
+    if constexpr (KIND == ROWS_WHOLE) {
 #pragma unroll
         for (int g = 0; g < V; g++) {
             uint32_t w0 = __byte_perm(codes(4 * g), codes(4 * g + 1), 0x5410), w1 = __byte_perm(codes(4 * g + 2), codes(4 * g + 3), 0x5410);
             if (!fine) w0 = w1 = 0;
             if (S::at(8 * g, 0) < p.K) *reinterpret_cast<uint2*>(out + S::at(8 * g, 0)) = make_uint2(w0, w1);
         }
+    } else if constexpr (KIND == ROWS_SHIFTED) {
+        // Whole words of codes: a thread's 8 begin d bytes before a word of the output, so its second word ends with the first d codes
+        // of the next lane.  What no word covers (between two warps, at the row's ends) goes byte by byte.
+        const int lane = threadIdx.x & 31;
+        auto bytes = [&](uint32_t w, int e, int n) {
+            for (int k = 0; k < n; k++, w >>= 8)
+                if (e + k >= 0 && e + k < p.K) out[e + k] = int8_t(w);
+        };
+#pragma unroll
+        for (int g = 0; g < V; g++) {
+            const int e = S::at(8 * g, shift), d = -int(reinterpret_cast<uintptr_t>(out + e)) & 3;
+            uint32_t w0 = __byte_perm(codes(4 * g), codes(4 * g + 1), 0x5410), w1 = __byte_perm(codes(4 * g + 2), codes(4 * g + 3), 0x5410);
+            if (!fine) w0 = w1 = 0;
+            const uint32_t w2 = __shfl_down_sync(0xffffffffu, w0, 1);
+            const uint32_t a = __funnelshift_r(w0, w1, 8 * d), b = __funnelshift_r(w1, w2, 8 * d);
+            if (!(lane > 0 && e + d - 4 >= 0 && e + d <= p.K)) bytes(w0, e, d);
+            if (e + d >= 0 && e + d + 4 <= p.K) *reinterpret_cast<uint32_t*>(out + e + d) = a;
+            else bytes(a, e + d, 4);
+            if (lane < 31 && e + d + 4 >= 0 && e + d + 8 <= p.K) *reinterpret_cast<uint32_t*>(out + e + d + 4) = b;
+            else bytes(b, e + d + 4, 4 - d);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 4 * V; i++) {
             const uint32_t c = fine ? codes(i) : 0u;
             const int e0 = S::at(2 * i, shift), e1 = S::at(2 * i + 1, shift);
-            if (e0 >= 0 && e0 < p.K) out[e0] = int8_t(c);
+            if (e0 < p.K) out[e0] = int8_t(c);
             if (e1 < p.K) out[e1] = int8_t(c >> 8);
         }
     }
 }
 
-template <typename T, int MODE, int V, int W, int THREADS>
+constexpr int rows_arrays(int mode) { return mode == ROWS_BLOCK ? 2 : 1; }         // row tensors read
+
+template <typename T, int MODE, int V, int KIND, int THREADS, int LAYOUT>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
-    using S = Slots<V, W>;
-    constexpr int P = 4 * V;                                      // pairs of elements of a thread
-    extern __shared__ __align__(16) uint8_t slots[];
-    __shared__ float2 part[2][2][32];
+    using S = Slots<V, KIND>;
+    constexpr bool STAGED = LAYOUT == ROWS_STAGED;
+    // the row's place in its CTA, uniform over a warp
+    const int ty = LAYOUT == ROWS_ONE ? 0 : __shfl_sync(0xffffffffu, int(threadIdx.y), 0), ny = LAYOUT == ROWS_ONE ? 1 : int(blockDim.y);
+    constexpr int P = S::P;                                       // pairs of elements of a thread
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float2 part[2][2][THREADS / 32];
     const int K = p.K;
-    const uint32_t slot_x = smem_u32(slots), slot_h = slot_x + blockDim.x * V * 16;
+    const uint32_t slot_bytes = blockDim.x * V * 16;
+    const uint32_t slot_x = smem_u32(smem) + ty * (rows_arrays(MODE) * slot_bytes), slot_h = slot_x + slot_bytes;
+    float* const staged_pre = reinterpret_cast<float*>(smem + ny * (rows_arrays(MODE) * slot_bytes));
+    float* const staged_post = staged_pre + S::staged_words(K);
+    float2* const my_part = &part[0][0][0] + ty * (blockDim.x / 32);      // of [2][2]: this row's warps
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // One pass over the grid: the next kernel may set itself up meanwhile.  Not beside a persistent grid: CTAs that come early take
+    // the first places that fall free, unevenly over the SMs, and their rows are dealt out already (rms_norm after rms_norm, 16384 x
+    // 7168: 84 us against 77 us).
+    if (int(gridDim.x) * ny >= p.M) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     auto row_of = [](const void* base, int64_t pitch, int row) { return static_cast<const uint16_t*>(base) + int64_t(row) * pitch; };
-    auto shift_of = [&](int row) { return W == 2 ? int(reinterpret_cast<uintptr_t>(row_of(p.x, p.ldx, row)) >> 1) & 1 : 0; };
-    // (r may be x: a row is written by the CTA that has read it)
+    auto shift_of = [&](int row) { return KIND == ROWS_SHIFTED ? int(reinterpret_cast<uintptr_t>(row_of(p.x, p.ldx, row)) >> 1) & 7 : 0; };
+    // (r may be x: a row is written by the threads that have read it)
     auto fetch = [&](int row, int shift) {
         if (MODE == ROWS_BLOCK) S::fetch(row_of(p.h, p.ldh, row), K, shift, slot_h);
         S::fetch(row_of(p.x, p.ldx, row), K, shift, slot_x);
     };
-    int row = blockIdx.x, shift = shift_of(row), turn = 0;
-    fetch(row, shift);
-    while (true) {
-        const int next = row + int(gridDim.x), next_shift = shift_of(next < p.M ? next : row);
+    const bool one_gate = p.gate && p.rows_per_gate >= p.M;
+    int row = blockIdx.x * ny + ty, turn = 0;
+    const int step = int(gridDim.x) * ny;
+    int shift = shift_of(row < p.M ? row : 0);
+    if (row < p.M) fetch(row, shift);
+    if constexpr (STAGED) {
+        const uint16_t* w_pre = static_cast<const uint16_t*>(p.w_pre);
+        const uint16_t* w_post = static_cast<const uint16_t*>(p.w_post);
+        const uint16_t* gate = static_cast<const uint16_t*>(p.gate);
+        const int margin = KIND == ROWS_SHIFTED ? 8 : 0;
+        for (int e = int(ty * blockDim.x + threadIdx.x) - margin; e < K + margin; e += int(blockDim.x) * ny) {
+            const bool in = e >= 0 && e < K;
+            const int at = S::staged_at(e, K);
+            if (p.w_pre) staged_pre[at] = in ? Pair<T>::lo(w_pre[e]) : 0.f;
+            if (MODE == ROWS_BLOCK) {
+                float c = in ? 1.f : 0.f;
+                if (in && p.w_post) c = Pair<T>::lo(w_post[e]);
+                if (in && one_gate) c *= Pair<T>::lo(gate[e]);
+                staged_post[at] = c;
+            }
+        }
+        __syncthreads();
+    }
+    while (row < p.M) {
+        const int next = row + step, next_shift = shift_of(next < p.M ? next : row);
+        float2* const red = my_part + turn * 2 * (THREADS / 32);
         uint32_t x[P];
         float s = 0.f, m = 0.f;
-        asm volatile("cp.async.wait_all;" ::: "memory");         // this thread reads only what it has fetched itself: no barrier
+        asm volatile("cp.async.wait_all;" ::: "memory");         // a thread reads only what it has fetched itself: no barrier
         S::take(slot_x, K, shift, x);
         if constexpr (MODE == ROWS_QUANT) {
             if (next < p.M) fetch(next, next_shift);
@@ -240,12 +335,18 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
 #pragma unroll
             for (int i = 0; i < P; i++) bits = __vmaxu2(bits, x[i] & 0x7fff7fffu);      // magnitudes order like their bits, NaN above all
             m = Pair<T>::lo(max(bits & 0xffffu, bits >> 16));
-            cta_reduce<false, true>(s, m, part[turn][0]);
-            quantize_row<V, W>(p, row, shift, m, [&](int i) { return up2<T>(x[i]); });
+            row_reduce<false, true, LAYOUT>(s, m, red);
+            quantize_row<V, KIND>(p, row, shift, m, [&](int i) { return up2<T>(x[i]); });
         } else {
-            F2 v[P];                                              // r * w_pre, then y
+            F2 v[P];                                              // r, r * w_pre, then y
             F2 sum = f2(0.f, 0.f);
             float rstd = 1.0f;
+            auto total = [&]() {
+                float lo, hi;
+                split(sum, lo, hi);
+                sum = f2(0.f, 0.f);
+                return lo + hi;
+            };
             if constexpr (MODE == ROWS_BLOCK) {
                 uint32_t h[P];
                 S::take(slot_h, K, shift, h);
@@ -255,30 +356,29 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
                 if (p.w_post) {
 #pragma unroll
                     for (int i = 0; i < P; i++) sum = fma2(v[i], v[i], sum);
-                    float s1;
-                    split(sum, s, s1);
-                    s += s1;
-                    cta_reduce<true, false>(s, m, part[turn][0]);
+                    s = total();
+                    row_reduce<true, false, LAYOUT>(s, m, red);
                     rstd = __frsqrt_rn(__fdiv_rn(s, float(K)) + p.eps);
-                    sum = f2(0.f, 0.f);
                 }
-                const uint16_t* gate = p.gate ? row_of(p.gate, p.ldg, row / p.rows_per_gate) : nullptr;
+                const F2 rstd2 = f2(rstd, rstd), scale2 = f2(p.residual_scale, p.residual_scale);
+                const uint16_t* gate = p.gate && !(STAGED && one_gate) ? row_of(p.gate, p.ldg, row / p.rows_per_gate) : nullptr;
 #pragma unroll
                 for (int g = 0; g < V; g++) {
-                    uint32_t w[4];
-                    if (p.w_post) {
-                        S::peek(static_cast<const uint16_t*>(p.w_post), K, shift, g, w);
+                    F2 w[4];
+                    if (STAGED || p.w_post) {
+                        if (STAGED) S::staged(staged_post, K, shift, g, w);
+                        else S::template peek<T>(p.w_post, K, shift, g, w);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) v[4 * g + i] = mul2(mul2(v[4 * g + i], f2(rstd, rstd)), up2<T>(w[i]));
+                        for (int i = 0; i < 4; i++) v[4 * g + i] = mul2(mul2(v[4 * g + i], rstd2), w[i]);
                     }
                     if (gate) {
-                        S::peek(gate, K, shift, g, w);
+                        S::template peek<T>(gate, K, shift, g, w);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) v[4 * g + i] = mul2(v[4 * g + i], up2<T>(w[i]));
+                        for (int i = 0; i < 4; i++) v[4 * g + i] = mul2(v[4 * g + i], w[i]);
                     }
 #pragma unroll
                     for (int i = 4 * g; i < 4 * g + 4; i++) {
-                        v[i] = fma2(f2(p.residual_scale, p.residual_scale), up2<T>(x[i]), v[i]);
+                        v[i] = fma2(scale2, up2<T>(x[i]), v[i]);
                         x[i] = down2<T>(v[i]);
                     }
                 }
@@ -288,64 +388,71 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
 #pragma unroll
                 for (int i = 0; i < P; i++) v[i] = up2<T>(x[i]);
             }
+            // (outside the row everything that v met is zero)
             if (MODE == ROWS_NORM || p.w_pre) {
 #pragma unroll
                 for (int g = 0; g < V; g++) {
-                    uint32_t w[4];
-                    S::peek(static_cast<const uint16_t*>(p.w_pre), K, shift, g, w);
+                    F2 w[4];
+                    if (STAGED) S::staged(staged_pre, K, shift, g, w);
+                    else S::template peek<T>(p.w_pre, K, shift, g, w);
 #pragma unroll
                     for (int i = 4 * g; i < 4 * g + 4; i++) {
-                        if (MODE == ROWS_BLOCK && W != 8) {
-                            // outside the row h and x are zeros, but the gates and weights that they met may be no numbers
-                            const int e0 = S::at(2 * i, shift), e1 = S::at(2 * i + 1, shift);
-                            float lo, hi;
-                            split(v[i], lo, hi);
-                            v[i] = f2(e0 >= 0 && e0 < K ? lo : 0.f, e1 < K ? hi : 0.f);
-                        }
                         sum = fma2(v[i], v[i], sum);
-                        v[i] = mul2(v[i], up2<T>(w[i - 4 * g]));
+                        v[i] = mul2(v[i], w[i - 4 * g]);
                         float lo, hi;
                         split(v[i], lo, hi);
                         m = max_abs3(m, lo, hi);
                     }
                 }
-                float s1;
-                split(sum, s, s1);
-                s += s1;
-                cta_reduce<true, true>(s, m, part[turn][1]);
+                s = total();
+                row_reduce<true, true, LAYOUT>(s, m, red + THREADS / 32);
                 rstd = __frsqrt_rn(__fdiv_rn(s, float(K)) + p.eps);
+                const F2 rstd2 = f2(rstd, rstd);
                 if (p.y) {
 #pragma unroll
-                    for (int i = 0; i < P; i++) x[i] = down2<T>(mul2(v[i], f2(rstd, rstd)));
+                    for (int i = 0; i < P; i++) x[i] = down2<T>(mul2(v[i], rstd2));
                     S::store(const_cast<uint16_t*>(row_of(p.y, p.ldy, row)), K, shift, x);
                 }
-                if (p.codes) quantize_row<V, W>(p, row, shift, m * rstd, [&](int i) { return mul2(v[i], f2(rstd, rstd)); });
+                if (p.codes) quantize_row<V, KIND>(p, row, shift, m * rstd, [&](int i) { return mul2(v[i], rstd2); });
             }
         }
-        if (next >= p.M) break;
         row = next; shift = next_shift; turn ^= 1;
     }
 }
 
-template <typename T, int MODE, int V, int W, int THREADS>
-static cudaError_t launch_rows_w(const RowsParams& p, int threads, int sm_count, cudaStream_t s) {
-    auto kern = rows_kernel<T, MODE, V, W, THREADS>;
-    const int smem = threads * V * 16 * (MODE == ROWS_BLOCK ? 2 : 1);
-    // CTAs of this size that an SM holds, asked for once for each device together with the shared memory
-    static std::atomic<int> held[64][THREADS / 32 + 1] = {};
+template <typename T, int MODE, int V, int KIND, int THREADS, int LAYOUT>
+static cudaError_t launch_rows_k(const RowsParams& p, int threads, int groups, int sm_count, cudaStream_t s) {
+    auto kern = rows_kernel<T, MODE, V, KIND, THREADS, LAYOUT>;
+    const int staged = LAYOUT == ROWS_STAGED ? (KIND == ROWS_SHIFTED ? (p.K + 24) / 8 * 9 : p.K) * 4 * rows_arrays(MODE) : 0;
+    const int smem = groups * threads * V * 16 * rows_arrays(MODE) + staged;
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    int per_sm = held[dev][threads / 32].load(std::memory_order_acquire);
-    if (per_sm == 0) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, THREADS * V * 16 * (MODE == ROWS_BLOCK ? 2 : 1));
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
-        if (e != cudaSuccess) return e;
-        held[dev][threads / 32].store(per_sm, std::memory_order_release);
+    static std::atomic<bool> attr_set[64] = {};
+    if (!attr_set[dev].load(std::memory_order_acquire)) {
+        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024); e != cudaSuccess) return e;
+        attr_set[dev].store(true, std::memory_order_release);
     }
+    // CTAs that an SM holds: asked for once for each device and size
+    static std::atomic<uint64_t> last[64] = {};
+    const uint64_t key = uint64_t(smem) << 24 | uint64_t(threads * groups) << 8;
+    uint64_t known = last[dev].load(std::memory_order_relaxed);
+    if ((known & ~uint64_t(255)) != key) {
+        int per_sm = 0;
+        if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads * groups, smem); e != cudaSuccess) return e;
+        known = key | uint64_t(per_sm);
+        last[dev].store(known, std::memory_order_relaxed);
+    }
+    // A norm that writes 16-bit rows back keeps no more than 48 KB of loads in flight on an SM: as many bytes are written as read, and
+    // more loads only make HBM turn more often (16384 x 7168: 3 rows 77.5 us, 4 rows 84.7 us; with int8 codes 65.7 against 59.9 us).
+    int held = int(known & 255);
+    if (MODE == ROWS_NORM && LAYOUT == ROWS_ONE && p.y && !p.codes) {
+        const int rows = 48 * 1024 / smem < 2 ? 2 : 48 * 1024 / smem;
+        if (held > rows) held = rows;
+    }
+    const int64_t fit = int64_t(sm_count) * held, want = (int64_t(p.M) + groups - 1) / groups;
     cudaLaunchConfig_t cfg = {};
-    const int64_t fit = int64_t(sm_count) * per_sm;
-    cfg.gridDim = dim3(unsigned(p.M < fit ? p.M : fit)); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.gridDim = dim3(unsigned(want < fit ? want : fit)); cfg.blockDim = dim3(threads, groups); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -353,28 +460,39 @@ static cudaError_t launch_rows_w(const RowsParams& p, int threads, int sm_count,
     return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
-template <typename T, int MODE, int V, int THREADS>
-static cudaError_t launch_rows_v(const RowsParams& p, int width, int threads, int sm_count, cudaStream_t s) {
-    switch (width) {
-        case 8: return launch_rows_w<T, MODE, V, 8, THREADS>(p, threads, sm_count, s);
-        case 2: return launch_rows_w<T, MODE, V, 2, THREADS>(p, threads, sm_count, s);
-        default: return launch_rows_w<T, MODE, V, 1, THREADS>(p, threads, sm_count, s);
+// Few rows: as many threads for a row as it has groups of 8 elements (up to 1024), since the time from the first load to the last
+// store counts.  Many rows: up to 4 groups for each thread, so that enough bytes are in flight and several rows share an SM.  Staging
+// the weights pays where a row meets two of them or reaches them unaligned: 16384 x 7168 block_norm 161 -> 156 us, 4098 x 5001 90 ->
+// 52 us, rms_norm 28.7 -> 24.9 us; an aligned rms_norm does better with its weights from L1 and more rows on an SM: 2048 x 8192 12.6
+// against 15.8 us.
+template <typename T, int MODE, int KIND>
+static cudaError_t launch_rows_m(const RowsParams& p, int sm_count, cudaStream_t s) {
+    const int n8 = (p.K + (KIND == ROWS_SHIFTED ? 7 : 0) + 7) / 8;
+    auto threads = [&](int v) { return ((n8 + v - 1) / v + 31) / 32 * 32; };
+    if (p.M <= 2 * sm_count && n8 <= 1024) return launch_rows_k<T, MODE, 1, KIND, 1024, ROWS_ONE>(p, threads(1), 1, sm_count, s);
+    if constexpr (MODE == ROWS_BLOCK || (MODE == ROWS_NORM && KIND != ROWS_WHOLE)) {
+        if (p.M <= 2 * sm_count) return launch_rows_k<T, MODE, 2, KIND, 1024, ROWS_ONE>(p, threads(2), 1, sm_count, s);
+        auto rows = [&](int v) { return 768 / threads(v) < 15 ? 768 / threads(v) : 15; };       // of a CTA (15: as many as it has barriers)
+        if (n8 <= 64) return launch_rows_k<T, MODE, 1, KIND, 768, ROWS_STAGED>(p, threads(1), rows(1), sm_count, s);
+        return launch_rows_k<T, MODE, 4, KIND, 768, ROWS_STAGED>(p, threads(4), rows(4), sm_count, s);
+    } else {
+        if (n8 <= 64) return launch_rows_k<T, MODE, 2, KIND, 256, ROWS_WARPS>(p, 32, 8, sm_count, s);        // a warp for each row
+        if (n8 <= 256) return launch_rows_k<T, MODE, 1, KIND, 256, ROWS_ONE>(p, threads(1), 1, sm_count, s);
+        if (n8 <= 512) return launch_rows_k<T, MODE, 2, KIND, 256, ROWS_ONE>(p, threads(2), 1, sm_count, s);
+        if (n8 <= 1024) return launch_rows_k<T, MODE, 4, KIND, 256, ROWS_ONE>(p, threads(4), 1, sm_count, s);
+        if (n8 <= 2048) return launch_rows_k<T, MODE, 4, KIND, 512, ROWS_ONE>(p, threads(4), 1, sm_count, s);
+        if constexpr (MODE == ROWS_QUANT) return launch_rows_k<T, MODE, 8, KIND, 1024, ROWS_ONE>(p, threads(8), 1, sm_count, s);
+        return cudaErrorInvalidValue;
     }
 }
 
-// Threads of a CTA and groups of 8 elements for each: few rows get many threads, since one row after the other counts; many rows
-// get up to 256, so that several CTAs share an SM and their reductions overlap.
 template <typename T, int MODE>
-static cudaError_t launch_rows_t(const RowsParams& p, int width, int sm_count, cudaStream_t s) {
-    const int groups = (p.K + (width == 2 ? 1 : 0) + 7) / 8;
-    auto threads = [&](int v) { return ((groups + v - 1) / v + 31) / 32 * 32; };
-    if (p.M <= 2 * sm_count && groups <= 1024) return launch_rows_v<T, MODE, 1, 1024>(p, width, threads(1), sm_count, s);
-    if (groups <= 256) return launch_rows_v<T, MODE, 1, 256>(p, width, threads(1), sm_count, s);
-    if (groups <= 512) return launch_rows_v<T, MODE, 2, 256>(p, width, threads(2), sm_count, s);
-    if (groups <= 1024) return launch_rows_v<T, MODE, 4, 256>(p, width, threads(4), sm_count, s);
-    if (groups <= 2049) return launch_rows_v<T, MODE, 4, 544>(p, width, threads(4), sm_count, s);       // (2049: 16384 elements from the middle of a word)
-    if constexpr (MODE == ROWS_QUANT) return launch_rows_v<T, MODE, 8, 1024>(p, width, threads(8), sm_count, s);
-    return cudaErrorInvalidValue;
+static cudaError_t launch_rows_t(const RowsParams& p, int kind, int sm_count, cudaStream_t s) {
+    switch (kind) {
+        case ROWS_WHOLE: return launch_rows_m<T, MODE, ROWS_WHOLE>(p, sm_count, s);
+        case ROWS_SHIFTED: return launch_rows_m<T, MODE, ROWS_SHIFTED>(p, sm_count, s);
+        default: return launch_rows_m<T, MODE, ROWS_SINGLE>(p, sm_count, s);
+    }
 }
 
 // ---- argument checks ------------------------------------------------------------------------
@@ -431,22 +549,21 @@ static int rows_call(const char* what, RowsParams p, int mode, int dtype, void* 
         for (int k = 0; k < i; k++)
             if (overlap(out[i], out[k], p.M)) return api_fail(TKB_ERR_INVALID_ARG, "%s: outputs %s and %s overlap", what, out[i].name, out[k].name);
     }
-    // 16-byte accesses where every row of every 16-bit tensor begins on 16 bytes (codes: on 8) and holds whole groups of 8; 4-byte
-    // ones where the rows of all of them begin alike within a word
+    // (a longest row that begins inside a group would need one group more than there are)
     const bool one = p.M == 1;
     auto whole = [&](const void* q, int64_t ld) { return !q || one || ld % 8 == 0; };
-    auto alike = [&](const void* q, int64_t ld) { return !q || (((reinterpret_cast<uintptr_t>(q) ^ reinterpret_cast<uintptr_t>(p.x)) & 2u) == 0 && (one || ((ld ^ p.ldx) & 1) == 0)); };
-    int width = 1;
+    auto alike = [&](const void* q, int64_t ld) { return !q || (((reinterpret_cast<uintptr_t>(q) ^ reinterpret_cast<uintptr_t>(p.x)) & 15u) == 0 && (one || ((ld ^ p.ldx) & 7) == 0)); };
+    int kind = ROWS_SINGLE;
     if ((bits & 15u) == 0 && p.K % 8 == 0 && whole(p.x, p.ldx) && whole(p.h, p.ldh) && whole(p.r, p.ldr) && whole(p.y, p.ldy) && whole(p.codes, p.ldc) &&
         (reinterpret_cast<uintptr_t>(p.codes) & 7u) == 0 && (!p.gate || p.M <= p.rows_per_gate || p.ldg % 8 == 0))
-        width = 8;
-    else if (p.K < kQuantMaxK && alike(p.h, p.ldh) && alike(p.r, p.ldr) && alike(p.y, p.ldy))
-        width = 2;
+        kind = ROWS_WHOLE;
+    else if (p.K + 7 <= max_k && alike(p.h, p.ldh) && alike(p.r, p.ldr) && alike(p.y, p.ldy))
+        kind = ROWS_SHIFTED;
     int sm_count; int* status;
     if (int e = api_device(&sm_count, &status)) return e;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-#define TKB_ROWS(MODE) (dtype == TKB_DTYPE_BF16 ? launch_rows_t<__nv_bfloat16, MODE>(p, width, sm_count, s) : launch_rows_t<__half, MODE>(p, width, sm_count, s))
+#define TKB_ROWS(MODE) (dtype == TKB_DTYPE_BF16 ? launch_rows_t<__nv_bfloat16, MODE>(p, kind, sm_count, s) : launch_rows_t<__half, MODE>(p, kind, sm_count, s))
     e = mode == ROWS_QUANT ? TKB_ROWS(ROWS_QUANT) : (mode == ROWS_NORM ? TKB_ROWS(ROWS_NORM) : TKB_ROWS(ROWS_BLOCK));
 #undef TKB_ROWS
     if (e != cudaSuccess) return api_fail(TKB_ERR_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
