@@ -58,13 +58,12 @@ template <> struct Pair<__half> {
     static __device__ __forceinline__ uint32_t down(float lo, float hi) { return pack_f16x2(lo, hi); }
 };
 // Two fp32 values in a register pair, which sm_100 adds and multiplies with one instruction
-struct F2 { uint64_t v; };
-__device__ __forceinline__ F2 f2(float lo, float hi) { F2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi)); return r; }
-__device__ __forceinline__ void split(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { F2 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return d; }
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) { F2 d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v)); return d; }
+typedef float2 F2;
+__device__ __forceinline__ F2 f2(float lo, float hi) { return make_float2(lo, hi); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) { return __fmul2_rn(a, b); }
 template <typename T> __device__ __forceinline__ F2 up2(uint32_t w) { return f2(Pair<T>::lo(w), Pair<T>::hi(w)); }
-template <typename T> __device__ __forceinline__ uint32_t down2(F2 a) { float lo, hi; split(a, lo, hi); return Pair<T>::down(lo, hi); }
+template <typename T> __device__ __forceinline__ uint32_t down2(F2 a) { return Pair<T>::down(a.x, a.y); }
 // max(|m|, |a|, |b|); a NaN stays one
 __device__ __forceinline__ float max_abs3(float m, float a, float b) { float d; asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(a), "f"(b)); return d; }
 
@@ -79,14 +78,20 @@ struct Slots {
     // address of words 4 g .. 4 g + 3 of the thread in a slot
     static __device__ __forceinline__ uint32_t word(uint32_t slot, int g) { return slot + (g * blockDim.x + threadIdx.x) * 16; }
 
-    // a row into the thread's own words of shared memory, asynchronously where a group is whole
+    // A row into the thread's own words of shared memory, asynchronously where a group is whole.  Groups outside the row hold zeros:
+    // they are cleared once, and one that lies in some rows and not in others is written anew for every row.
+    static __device__ __forceinline__ void clear(int K, uint32_t slot) {
+#pragma unroll
+        for (int g = 0; g < V; g++)
+            if (at(8 * g, 0) >= K) st_shared_v4(word(slot, g), 0u, 0u, 0u, 0u);
+    }
     static __device__ __forceinline__ void fetch(const uint16_t* row, int K, int shift, uint32_t slot) {
 #pragma unroll
         for (int g = 0; g < V; g++) {
             const int e = at(8 * g, shift);
             if (KIND == ROWS_WHOLE ? e < K : (KIND == ROWS_SHIFTED && e >= 0 && e + 8 <= K)) {
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(word(slot, g)), "l"(row + e) : "memory");
-            } else if (KIND != ROWS_WHOLE && e < K) {
+            } else if (KIND != ROWS_WHOLE && e < K + 8) {
                 uint32_t w[4];
                 gather(row, K, shift, g, w);
                 st_shared_v4(word(slot, g), w[0], w[1], w[2], w[3]);
@@ -96,12 +101,6 @@ struct Slots {
     }
     // the elements of group g that lie in the row, one by one; zeros for the others
     static __device__ __forceinline__ void gather(const uint16_t* row, int K, int shift, int g, uint32_t (&w)[4]) {
-        if (KIND == ROWS_SHIFTED && at(8 * g, shift) >= 0 && at(8 * g, shift) + 8 <= K) {
-            const uint16_t* q = row + at(8 * g, shift);
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = q[2 * i] | uint32_t(q[2 * i + 1]) << 16;
-            return;
-        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int e0 = at(8 * g + 2 * i, shift), e1 = at(8 * g + 2 * i + 1, shift);
@@ -109,16 +108,13 @@ struct Slots {
             if (e1 >= 0 && e1 < K) w[i] |= uint32_t(row[e1]) << 16;
         }
     }
-    static __device__ __forceinline__ void take(uint32_t slot, int K, int shift, uint32_t (&w)[P]) {
+    static __device__ __forceinline__ void take(uint32_t slot, uint32_t (&w)[P]) {
 #pragma unroll
-        for (int g = 0; g < V; g++) {
-            w[4 * g] = w[4 * g + 1] = w[4 * g + 2] = w[4 * g + 3] = 0;
-            if (at(8 * g, shift) < K)
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(w[4 * g]), "=r"(w[4 * g + 1]), "=r"(w[4 * g + 2]), "=r"(w[4 * g + 3])
-                             : "r"(word(slot, g))
-                             : "memory");
-        }
+        for (int g = 0; g < V; g++)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[4 * g]), "=r"(w[4 * g + 1]), "=r"(w[4 * g + 2]), "=r"(w[4 * g + 3])
+                         : "r"(word(slot, g))
+                         : "memory");
     }
     static __device__ __forceinline__ void store(uint16_t* row, int K, int shift, const uint32_t (&w)[P]) {
 #pragma unroll
@@ -136,51 +132,43 @@ struct Slots {
             }
         }
     }
-    // group g of a vector that every row meets (weights, gates), from L1, and again where it is needed again
+    // group g of a vector that rows meet (weights, gates), from L1, and again where it is needed again; zeros outside the row
     template <typename T>
     static __device__ __forceinline__ void peek(const void* vec, int K, int shift, int g, F2 (&w)[4]) {
         uint32_t b[4] = {0u, 0u, 0u, 0u};
         const uint16_t* v = static_cast<const uint16_t*>(vec);
+        const int e = at(8 * g, shift);
         if constexpr (KIND == ROWS_WHOLE) {
-            if (at(8 * g, 0) < K) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "l"(v + at(8 * g, 0)));
+            if (e < K) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "l"(v + e));
+        } else if (KIND == ROWS_SHIFTED && e >= 0 && e + 8 <= K) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) b[i] = __ldg(v + e + 2 * i) | uint32_t(__ldg(v + e + 2 * i + 1)) << 16;
         } else {
             gather(v, K, shift, g, b);
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) w[i] = up2<T>(b[i]);
     }
-    // The same from shared memory as fp32.  Layouts without bank conflicts: WHOLE two halves, of the first and last 4 of every group
-    // (16-byte accesses); SHIFTED one word of padding for every 8, with 8 zeros before and behind the row.
-    static __device__ __forceinline__ int staged_words(int K) { return KIND == ROWS_WHOLE ? K : (KIND == ROWS_SHIFTED ? (K + 24) / 8 * 9 : K); }
-    static __device__ __forceinline__ int staged_at(int e, int K) {
-        return KIND == ROWS_WHOLE ? ((e >> 2) & 1) * (K / 2) + (e >> 3) * 4 + (e & 3) : (KIND == ROWS_SHIFTED ? e + 8 + ((e + 8) >> 3) : e);
+    // The same from shared memory as fp32, for the elements of all threads (zeros outside the row).  Layouts without bank conflicts:
+    // WHOLE two halves, of the first and last 4 of every group (16-byte accesses); SHIFTED one word of padding for every 8.
+    static __host__ __device__ __forceinline__ int staged_words(int threads) { return KIND == ROWS_SHIFTED ? (threads * V + 1) * 9 : threads * V * 8; }
+    static __device__ __forceinline__ int staged_at(int e) {
+        const int half = int(blockDim.x) * V * 4;
+        return KIND == ROWS_WHOLE ? ((e >> 2) & 1) * half + (e >> 3) * 4 + (e & 3) : (KIND == ROWS_SHIFTED ? e + 8 + ((e + 8) >> 3) : e);
     }
-    static __device__ __forceinline__ void staged(const float* vec, int K, int shift, int g, F2 (&w)[4]) {
+    static __device__ __forceinline__ void staged(const float* vec, int shift, int g, F2 (&w)[4]) {
+        const int c = int(threadIdx.x) + g * int(blockDim.x);
         if constexpr (KIND == ROWS_WHOLE) {
-            const int e = at(8 * g, 0);
-            float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-            if (e < K) {
-                a = *reinterpret_cast<const float4*>(vec + e / 2);
-                b = *reinterpret_cast<const float4*>(vec + K / 2 + e / 2);
-            }
+            const float4 a = *reinterpret_cast<const float4*>(vec + c * 4), b = *reinterpret_cast<const float4*>(vec + int(blockDim.x) * V * 4 + c * 4);
             w[0] = f2(a.x, a.y); w[1] = f2(a.z, a.w); w[2] = f2(b.x, b.y); w[3] = f2(b.z, b.w);
+        } else if constexpr (KIND == ROWS_SHIFTED) {
+            // staged_at(8 c - shift + j) = 9 (c + 1) - shift + j - (j < shift): one address for all but `shift`
+            const float* q = vec + 9 * (c + 1) - shift;
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = f2(q[2 * i - (2 * i < shift)], q[2 * i + 1 - (2 * i + 1 < shift)]);
         } else {
-            if constexpr (KIND == ROWS_SHIFTED) {
-                // staged_at(8 c - shift + j) = 9 (c + 1) - shift + j - (j < shift), c the group's number: one address for all but `shift`
-                const float* q = vec + 9 * (int(threadIdx.x) + g * int(blockDim.x) + 1) - shift;
-                const bool in = at(8 * g, shift) < K;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int j0 = 2 * i - (2 * i < shift), j1 = 2 * i + 1 - (2 * i + 1 < shift);
-                    w[i] = in ? f2(q[j0], q[j1]) : f2(0.f, 0.f);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int e0 = at(8 * g + 2 * i, shift), e1 = at(8 * g + 2 * i + 1, shift);
-                    w[i] = f2(e0 < K ? vec[e0] : 0.f, e1 < K ? vec[e1] : 0.f);
-                }
-            }
+            for (int i = 0; i < 4; i++) w[i] = f2(vec[at(8 * g + 2 * i, 0)], vec[at(8 * g + 2 * i + 1, 0)]);
         }
     }
 };
@@ -227,9 +215,8 @@ __device__ __forceinline__ void quantize_row(const RowsParams& p, int row, int s
     const F2 inv2 = f2(inv, inv), grid = f2(12582912.0f, 12582912.0f);
     // the codes of pair i in bits 0-7 and 8-15
     auto codes = [&](int i) {
-        float lo, hi;
-        split(fma2(value(i), inv2, grid), lo, hi);
-        return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x0040);
+        const F2 c = fma2(value(i), inv2, grid);
+        return __byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x0040);
     };
     if constexpr (KIND == ROWS_WHOLE) {
 #pragma unroll
@@ -285,7 +272,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
     const uint32_t slot_bytes = blockDim.x * V * 16;
     const uint32_t slot_x = smem_u32(smem) + ty * (rows_arrays(MODE) * slot_bytes), slot_h = slot_x + slot_bytes;
     float* const staged_pre = reinterpret_cast<float*>(smem + ny * (rows_arrays(MODE) * slot_bytes));
-    float* const staged_post = staged_pre + S::staged_words(K);
+    float* const staged_post = staged_pre + S::staged_words(blockDim.x);
     float2* const my_part = &part[0][0][0] + ty * (blockDim.x / 32);      // of [2][2]: this row's warps
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // One pass over the grid: the next kernel may set itself up meanwhile.  Not beside a persistent grid: CTAs that come early take
@@ -303,15 +290,17 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
     int row = blockIdx.x * ny + ty, turn = 0;
     const int step = int(gridDim.x) * ny;
     int shift = shift_of(row < p.M ? row : 0);
+    S::clear(K, slot_x);
+    if (MODE == ROWS_BLOCK) S::clear(K, slot_h);
     if (row < p.M) fetch(row, shift);
     if constexpr (STAGED) {
         const uint16_t* w_pre = static_cast<const uint16_t*>(p.w_pre);
         const uint16_t* w_post = static_cast<const uint16_t*>(p.w_post);
         const uint16_t* gate = static_cast<const uint16_t*>(p.gate);
-        const int margin = KIND == ROWS_SHIFTED ? 8 : 0;
-        for (int e = int(ty * blockDim.x + threadIdx.x) - margin; e < K + margin; e += int(blockDim.x) * ny) {
+        const int first = KIND == ROWS_SHIFTED ? -8 : 0, last = int(blockDim.x) * V * 8;
+        for (int e = int(ty * blockDim.x + threadIdx.x) + first; e < last; e += int(blockDim.x) * ny) {
             const bool in = e >= 0 && e < K;
-            const int at = S::staged_at(e, K);
+            const int at = S::staged_at(e);
             if (p.w_pre) staged_pre[at] = in ? Pair<T>::lo(w_pre[e]) : 0.f;
             if (MODE == ROWS_BLOCK) {
                 float c = in ? 1.f : 0.f;
@@ -328,7 +317,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
         uint32_t x[P];
         float s = 0.f, m = 0.f;
         asm volatile("cp.async.wait_all;" ::: "memory");         // a thread reads only what it has fetched itself: no barrier
-        S::take(slot_x, K, shift, x);
+        S::take(slot_x, x);
         if constexpr (MODE == ROWS_QUANT) {
             if (next < p.M) fetch(next, next_shift);
             uint32_t bits = 0;
@@ -342,14 +331,13 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
             F2 sum = f2(0.f, 0.f);
             float rstd = 1.0f;
             auto total = [&]() {
-                float lo, hi;
-                split(sum, lo, hi);
+                const float t = sum.x + sum.y;
                 sum = f2(0.f, 0.f);
-                return lo + hi;
+                return t;
             };
             if constexpr (MODE == ROWS_BLOCK) {
                 uint32_t h[P];
-                S::take(slot_h, K, shift, h);
+                S::take(slot_h, h);
                 if (next < p.M) fetch(next, next_shift);
 #pragma unroll
                 for (int i = 0; i < P; i++) v[i] = up2<T>(h[i]);
@@ -366,7 +354,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
                 for (int g = 0; g < V; g++) {
                     F2 w[4];
                     if (STAGED || p.w_post) {
-                        if (STAGED) S::staged(staged_post, K, shift, g, w);
+                        if (STAGED) S::staged(staged_post, shift, g, w);
                         else S::template peek<T>(p.w_post, K, shift, g, w);
 #pragma unroll
                         for (int i = 0; i < 4; i++) v[4 * g + i] = mul2(mul2(v[4 * g + i], rstd2), w[i]);
@@ -393,15 +381,13 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
 #pragma unroll
                 for (int g = 0; g < V; g++) {
                     F2 w[4];
-                    if (STAGED) S::staged(staged_pre, K, shift, g, w);
+                    if (STAGED) S::staged(staged_pre, shift, g, w);
                     else S::template peek<T>(p.w_pre, K, shift, g, w);
 #pragma unroll
                     for (int i = 4 * g; i < 4 * g + 4; i++) {
                         sum = fma2(v[i], v[i], sum);
                         v[i] = mul2(v[i], w[i - 4 * g]);
-                        float lo, hi;
-                        split(v[i], lo, hi);
-                        m = max_abs3(m, lo, hi);
+                        m = max_abs3(m, v[i].x, v[i].y);
                     }
                 }
                 s = total();
@@ -420,10 +406,16 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
     }
 }
 
+// Whether a call writes as many bytes as it reads and more than L2 takes up.  More loads in flight then only make HBM turn more
+// often: 16384 x 7168 rms_norm with 3 rows on an SM 72 us, with 4 rows 84 us; block_norm with 2 rows 158 us, with 3 rows 175 us (and
+// with int8 results, which write half, 65 against 60 us and 158 against 131 us).  So such calls keep about 48 KB (two row tensors: 64 KB)
+// in flight on an SM.
+static bool rows_turn(const RowsParams& p) { return p.y && !p.codes && int64_t(p.M) * p.K * (p.h ? 8 : 4) > (int64_t(256) << 20); }
+
 template <typename T, int MODE, int V, int KIND, int THREADS, int LAYOUT>
 static cudaError_t launch_rows_k(const RowsParams& p, int threads, int groups, int sm_count, cudaStream_t s) {
     auto kern = rows_kernel<T, MODE, V, KIND, THREADS, LAYOUT>;
-    const int staged = LAYOUT == ROWS_STAGED ? (KIND == ROWS_SHIFTED ? (p.K + 24) / 8 * 9 : p.K) * 4 * rows_arrays(MODE) : 0;
+    const int staged = LAYOUT == ROWS_STAGED ? Slots<V, KIND>::staged_words(threads) * 4 * rows_arrays(MODE) : 0;
     const int smem = groups * threads * V * 16 * rows_arrays(MODE) + staged;
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
@@ -443,10 +435,8 @@ static cudaError_t launch_rows_k(const RowsParams& p, int threads, int groups, i
         known = key | uint64_t(per_sm);
         last[dev].store(known, std::memory_order_relaxed);
     }
-    // A norm that writes 16-bit rows back keeps no more than 48 KB of loads in flight on an SM: as many bytes are written as read, and
-    // more loads only make HBM turn more often (16384 x 7168: 3 rows 77.5 us, 4 rows 84.7 us; with int8 codes 65.7 against 59.9 us).
     int held = int(known & 255);
-    if (MODE == ROWS_NORM && LAYOUT == ROWS_ONE && p.y && !p.codes) {
+    if (MODE == ROWS_NORM && LAYOUT == ROWS_ONE && rows_turn(p)) {
         const int rows = 48 * 1024 / smem < 2 ? 2 : 48 * 1024 / smem;
         if (held > rows) held = rows;
     }
@@ -472,7 +462,10 @@ static cudaError_t launch_rows_m(const RowsParams& p, int sm_count, cudaStream_t
     if (p.M <= 2 * sm_count && n8 <= 1024) return launch_rows_k<T, MODE, 1, KIND, 1024, ROWS_ONE>(p, threads(1), 1, sm_count, s);
     if constexpr (MODE == ROWS_BLOCK || (MODE == ROWS_NORM && KIND != ROWS_WHOLE)) {
         if (p.M <= 2 * sm_count) return launch_rows_k<T, MODE, 2, KIND, 1024, ROWS_ONE>(p, threads(2), 1, sm_count, s);
-        auto rows = [&](int v) { return 768 / threads(v) < 15 ? 768 / threads(v) : 15; };       // of a CTA (15: as many as it has barriers)
+        auto rows = [&](int v) {                                 // of a CTA (15: as many as it has barriers)
+            const int fit = 768 / threads(v) < 15 ? 768 / threads(v) : 15, turn = 64 * 1024 / (threads(v) * v * 16 * rows_arrays(MODE));
+            return rows_turn(p) && turn < fit ? (turn < 1 ? 1 : turn) : fit;
+        };
         if (n8 <= 64) return launch_rows_k<T, MODE, 1, KIND, 768, ROWS_STAGED>(p, threads(1), rows(1), sm_count, s);
         return launch_rows_k<T, MODE, 4, KIND, 768, ROWS_STAGED>(p, threads(4), rows(4), sm_count, s);
     } else {
