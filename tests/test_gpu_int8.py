@@ -174,9 +174,9 @@ def test_gemm_repeats_bit_for_bit(cuda, lib):
         assert torch.equal(D[0], D[1]) and torch.equal(D[0], D[2])
 
 
-@pytest.mark.parametrize("M,N,K", [(1, 96, 2048), (5, 2048, 1024), (33, 77, 2000), (65, 77, 2000), (128, 1000, 4096)])
-def test_gemm_split_over_a_cluster_many_times(cuda, lib, M, N, K):
-    """K split over the CTAs of a cluster, back to back: every launch exchanges its sums before the next one begins."""
+@pytest.mark.parametrize("M,N,K", [(1, 96, 2048), (5, 2048, 1024), (33, 77, 2000), (65, 77, 2000), (128, 1000, 4096), (7, 6000, 1040), (100, 5000, 528)])
+def test_gemm_of_few_tokens_many_times(cuda, lib, M, N, K):
+    """Back to back, each launch beginning while the one before it ends."""
     a, a_sc, b, b_sc = _operands(M, N, K, cuda, seed=8)
     D = [torch.full((M, N), float("nan"), device=cuda) for _ in range(40)]
     for _ in range(10):

@@ -96,7 +96,7 @@ struct GemmParams {
     // reduce-scatter epilogue (MODE_RS): tensor maps (device memory) of every rank's output rows, rows per rank
     const CUtensorMap* rs_maps; int rs_rows;
     // KIND_INT8: output type and, for outputs that TMA cannot address, where to store without it
-    int out_dtype, plain_out; void* D; int64_t ldd;
+    int out_dtype; void* D; int64_t ldd;
 };
 
 // NVFP4 quantization of one 16-value block held as 8 packed bf16 pairs, with the IEEE arithmetic of the standalone
@@ -127,30 +127,17 @@ __device__ __forceinline__ uint8_t quant_block16(const uint32_t (&w)[8], float s
     return s8;
 }
 
-// Epilogue of KIND_INT8 for one warp: 32 rows x 64 columns of int32 sums (this thread: row row0 + lane) are scaled, converted
-// and leave through the warp's staging box (rows of 128 bytes, 128-byte swizzle): one box of 64 columns for the 16-bit types,
-// two of 32 columns for fp32.  The sums are converted to fp32 first (one rounding above 2^24), then multiplied by the row's and
-// by the column's scale.  A box leaves by TMA, which clips the edges of D, or, where D's base or pitch is not a multiple of 16
-// bytes, row by row with one element per lane.
-__device__ __forceinline__ void int8_epilogue(uint32_t (&r)[64], const CUtensorMap* tmD, const GemmParams& p, uint32_t stage_box, int row0, int col0,
+// Epilogue of KIND_INT8 for one warp: 32 rows x 64 columns of int32 sums (this thread: row row0 + lane) from tensor memory are scaled,
+// converted and leave through the warp's staging box (rows of 128 bytes, 128-byte swizzle): one box of 64 columns for the 16-bit
+// types, two of 32 columns for fp32.  The sums are converted to fp32 first (one rounding above 2^24), then multiplied by the row's
+// and by the column's scale.  A box leaves by TMA, which clips the edges of D, or (DIRECT), where D's base or pitch is not a multiple
+// of 16 bytes, row by row with one element per lane.
+template <bool DIRECT>
+__device__ __forceinline__ void int8_epilogue(uint32_t acc_t, const CUtensorMap* tmD, const GemmParams& p, uint32_t stage_box, int row0, int col0,
                                               float row_scale, int lane, uint64_t policy) {
     if (row0 >= p.M || col0 >= p.N) return;                  // uniform over the warp
-    const float* cs = p.sgB + col0;
-    if (col0 + 64 <= p.N && (reinterpret_cast<uintptr_t>(cs) & 15u) == 0) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float4 c = __ldg(reinterpret_cast<const float4*>(cs) + i);      // the same address in all lanes
-            r[4 * i] = __float_as_uint(__int2float_rn(int(r[4 * i])) * row_scale * c.x);
-            r[4 * i + 1] = __float_as_uint(__int2float_rn(int(r[4 * i + 1])) * row_scale * c.y);
-            r[4 * i + 2] = __float_as_uint(__int2float_rn(int(r[4 * i + 2])) * row_scale * c.z);
-            r[4 * i + 3] = __float_as_uint(__int2float_rn(int(r[4 * i + 3])) * row_scale * c.w);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 64; i++) r[i] = __float_as_uint(__int2float_rn(int(r[i])) * row_scale * __ldg(cs + min(i, p.N - 1 - col0)));
-    }
     auto leave = [&](int col, int elem_bytes) {              // the box holds columns col .. col + 128 / elem_bytes - 1
-        if (!p.plain_out) {
+        if constexpr (!DIRECT) {
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
@@ -160,52 +147,78 @@ __device__ __forceinline__ void int8_epilogue(uint32_t (&r)[64], const CUtensorM
             return;
         }
         __syncwarp();
+        // 8 rows at a time, so that their loads and stores are in flight together
         const int rows = min(32, p.M - row0);
-        for (int row = 0; row < rows; row++) {
-            uint8_t* out = static_cast<uint8_t*>(p.D) + (int64_t(row0 + row) * p.ldd + col) * elem_bytes;
-            for (int e = lane; e < 128 / elem_bytes && col + e < p.N; e += 32) {
-                const uint32_t at = uint32_t(e) * elem_bytes;
-                const uint32_t src = stage_box + row * 128 + (((at >> 4) ^ (row & 7)) << 4) + (at & 15u);
+        const bool in0 = col + lane < p.N, in1 = col + lane + 32 < p.N;
+        for (int row = 0; row < rows; row += 8) {
+            uint32_t v[8][2];
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t at = uint32_t(lane + 32 * h) * elem_bytes;
+                    const uint32_t src = stage_box + (row + k) * 128 + ((((at >> 4) & 7u) ^ uint32_t((row + k) & 7)) << 4) + (at & 15u);
+                    if (elem_bytes == 2) { uint16_t u; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(src) : "memory"); v[k][h] = u; }
+                    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[k][h]) : "r"(src) : "memory");
+                }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if (row + k >= rows) continue;
+                const int64_t at = int64_t(row0 + row + k) * p.ldd + col + lane;
                 if (elem_bytes == 2) {
-                    uint16_t v;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(src));
-                    reinterpret_cast<uint16_t*>(out)[e] = v;
-                } else {
-                    uint32_t v;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(src));
-                    reinterpret_cast<uint32_t*>(out)[e] = v;
+                    if (in0) static_cast<uint16_t*>(p.D)[at] = uint16_t(v[k][0]);
+                    if (in1) static_cast<uint16_t*>(p.D)[at + 32] = uint16_t(v[k][1]);
+                } else if (in0) {                            // (an fp32 box has 32 columns)
+                    static_cast<uint32_t*>(p.D)[at] = v[k][0];
                 }
             }
         }
     };
     auto box_free = [&]() {                                  // the box's previous contents have been read
-        if (!p.plain_out && lane == 0) tma_store_wait_read<0>();
+        if (!DIRECT && lane == 0) tma_store_wait_read<0>();
         __syncwarp();
     };
     const uint32_t box_row = stage_box + lane * 128;
-    if (p.out_dtype == TKB_DTYPE_FP32) {
+    const bool fp32 = p.out_dtype == TKB_DTYPE_FP32, fp16 = p.out_dtype == TKB_DTYPE_FP16;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            if (col0 + 32 * h >= p.N) return;
+    for (int h = 0; h < 2; h++) {                            // 32 columns at a time
+        const int col = col0 + 32 * h;
+        if (fp32 && col >= p.N) return;
+        uint32_t r[32];
+        __syncwarp();
+        tmem_ld_32x32(acc_t + 32 * h, r);
+        tmem_ld_wait();
+        const float* cs = p.sgB + col;
+        if (col + 32 <= p.N && (reinterpret_cast<uintptr_t>(cs) & 15u) == 0) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float4 c = __ldg(reinterpret_cast<const float4*>(cs) + i);      // the same address in all lanes
+                r[4 * i] = __float_as_uint(__int2float_rn(int(r[4 * i])) * row_scale * c.x);
+                r[4 * i + 1] = __float_as_uint(__int2float_rn(int(r[4 * i + 1])) * row_scale * c.y);
+                r[4 * i + 2] = __float_as_uint(__int2float_rn(int(r[4 * i + 2])) * row_scale * c.z);
+                r[4 * i + 3] = __float_as_uint(__int2float_rn(int(r[4 * i + 3])) * row_scale * c.w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__int2float_rn(int(r[i])) * row_scale * __ldg(p.sgB + min(col + i, p.N - 1)));
+        }
+        if (fp32) {
             box_free();
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                st_shared_v4(box_row + ((j ^ (lane & 7)) << 4), r[32 * h + 4 * j], r[32 * h + 4 * j + 1], r[32 * h + 4 * j + 2], r[32 * h + 4 * j + 3]);
-            leave(col0 + 32 * h, 4);
+            for (int j = 0; j < 8; j++) st_shared_v4(box_row + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+            leave(col, 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float lo = __uint_as_float(r[2 * i]), hi = __uint_as_float(r[2 * i + 1]);
+                r[i] = fp16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+            }
+            if (h == 0) box_free();
+#pragma unroll
+            for (int j = 0; j < 4; j++) st_shared_v4(box_row + (((4 * h + j) ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+            if (h == 1) leave(col0, 2);
         }
-        return;
     }
-    if (p.out_dtype == TKB_DTYPE_FP16) {
-#pragma unroll
-        for (int i = 0; i < 32; i++) r[i] = pack_f16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; i++) r[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-    }
-    box_free();
-#pragma unroll
-    for (int j = 0; j < 8; j++) st_shared_v4(box_row + ((j ^ (lane & 7)) << 4), r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-    leave(col0, 2);
 }
 
 // All-gather mode (tensor-parallel GEMM): the A operand is row-sharded over `world` GPUs.  Every rank
@@ -810,6 +823,21 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             wait_tf += t1 - t0;
             tile_count++;
             tc_fence_after();
+            if constexpr (KIND == KIND_INT8) {
+                const int row0 = m_blk * C::BM + int(cta_rank) * 128 + quarter * 32;
+                const int col0 = n_blk * BN + col_base;
+                const uint32_t acc_t = tmem_base + (uint32_t(quarter * 32) << 16) + buf * C::ACC_COLS + col_base;
+                int8_epilogue<MODE == MODE_DIRECT>(acc_t, &tmD, p, stage_box, row0, col0, row_scale, lane, d_policy);
+                int8_epilogue<MODE == MODE_DIRECT>(acc_t + 64, &tmD, p, stage_box, row0, col0 + 64, row_scale, lane, d_policy);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {                             // (two accumulators: the next tile's MMAs are under way)
+                    const uint32_t tmem_empty_leader = buf ? tmem_empty_leader1 : tmem_empty_leader0;
+                    if constexpr (CTAS == 2) mbar_arrive_cluster(tmem_empty_leader); else mbar_arrive(tmem_empty_leader);
+                }
+                drain += clock64() - t1;
+                continue;
+            }
             // Drain: both halves of this warp's 128 accumulator columns are requested back to back and only waited
             // for once; tensor memory goes back to the MMA warp before any arithmetic on the values.
 #pragma unroll
@@ -823,13 +851,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             if (lane == 0 && mh == MH - 1) {                 // the last half is in registers: tensor memory goes back
                 const uint32_t tmem_empty_leader = buf ? tmem_empty_leader1 : tmem_empty_leader0;
                 if constexpr (CTAS == 2) mbar_arrive_cluster(tmem_empty_leader); else mbar_arrive(tmem_empty_leader);
-            }
-            if constexpr (KIND == KIND_INT8) {
-                const int row0 = m_blk * C::BM + int(cta_rank) * 128 + quarter * 32;
-                const int col0 = n_blk * BN + col_base;
-                int8_epilogue(r0, &tmD, p, stage_box, row0, col0, row_scale, lane, d_policy);
-                int8_epilogue(r1, &tmD, p, stage_box, row0, col0 + 64, row_scale, lane, d_policy);
-                continue;
             }
             uint32_t packed[C::COLS_PER_EPI_WARP / 2];
 #pragma unroll
@@ -994,7 +1015,7 @@ static cudaError_t launch_t(const GemmArgs& a) {
     static const int group_env = getenv("TKB_GEMM_GROUP") ? atoi(getenv("TKB_GEMM_GROUP")) : 0;
     GemmParams p{a.sgA, a.sgB, a.M, a.N, a.K, group_env > 0 ? group_env : 16, 0, a.status, a.prof, api_wait_limit(),
                  static_cast<uint8_t*>(a.q_codes), static_cast<uint8_t*>(a.q_sc), a.q_sg, a.q_amax, a.q_arith, a.rs_maps, a.rs_rows_per_rank,
-                 a.out_dtype, a.plain_out, a.D, a.ldd};
+                 a.out_dtype, a.D, a.ldd};
     if (MODE == MODE_RS && a.rs_world > 0) {
         // start with the rows of the next rank, so that the ranks do not all add into the same owner at the same time
         p.group = a.rs_rows_per_rank / C::BM;
@@ -1003,16 +1024,16 @@ static cudaError_t launch_t(const GemmArgs& a) {
     return cudaLaunchKernelEx(&cfg, kern, a.tmA, a.tmB, a.tmSA, a.tmSB, a.tmD, p, a.comm);
 }
 
-template <int KIND>
+template <int KIND, int MODE = MODE_PLAIN>
 static cudaError_t launch_k(const GemmArgs& a) {
     if constexpr (KIND == KIND_BF16 || KIND == KIND_FP8) {
         if (a.config & 4) return launch_t<KIND, 2, 256, MODE_PLAIN, 2>(a);      // 512 x 256 cluster tiles
     }
     switch (a.config & 3) {
-        case 0: return launch_t<KIND, 2, 256>(a);
-        case 1: return launch_t<KIND, 1, 256>(a);
-        case 2: return launch_t<KIND, 2, 128>(a);
-        default: return launch_t<KIND, 1, 128>(a);
+        case 0: return launch_t<KIND, 2, 256, MODE>(a);
+        case 1: return launch_t<KIND, 1, 256, MODE>(a);
+        case 2: return launch_t<KIND, 2, 128, MODE>(a);
+        default: return launch_t<KIND, 1, 128, MODE>(a);
     }
 }
 
@@ -1038,7 +1059,7 @@ cudaError_t launch_gemm(const GemmArgs& a) {
         case KIND_MXFP8: return launch_k<KIND_MXFP8>(a);
         case KIND_NVFP4: return launch_k<KIND_NVFP4>(a);
         case KIND_FP8: return launch_k<KIND_FP8>(a);
-        case KIND_INT8: return launch_k<KIND_INT8>(a);
+        case KIND_INT8: return a.mode == MODE_DIRECT ? launch_k<KIND_INT8, MODE_DIRECT>(a) : launch_k<KIND_INT8>(a);
         default: return cudaErrorInvalidValue;
     }
 }

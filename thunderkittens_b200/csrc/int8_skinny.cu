@@ -1,16 +1,19 @@
-// Skinny-M ("decode") 8-bit integer GEMM: D[M, N] = A_sc[m] * B_sc[n] * sum_k A[m, k] * B[n, k] with M <= 128.
+// 8-bit integer GEMM with few tokens ("decode"): D[M, N] = A_sc[m] * B_sc[n] * sum_k A[m, k] * B[n, k] with M <= 128.
 //
-// Bound by streaming the N * K bytes of weights from HBM once.  Operands are swapped as in the NVFP4 decode kernel (decode.cu):
-// weight rows are the MMA's M side (128 lanes), the tokens, padded to 16 / 32 / 64 / 128, its N side.  What matters is that every
-// SM streams the same number of bytes without a gap:
+// Bound by streaming the N * K bytes of weights from HBM once.  Two kernels, neither of which shares anything between CTAs or leaves
+// anything but D in global memory, so that calls on any number of streams and captured graphs do not meet:
+//
+// Long streams: operands are swapped as in the NVFP4 decode kernel (decode.cu): weight rows are the M side of a tcgen05.mma (128
+// lanes), the tokens, padded to 16 / 32 / 64 / 128, its N side.  What matters is that every SM streams the same number of bytes
+// without a gap:
 //   * slabs have R <= 128 weight rows, R chosen so that they divide evenly over the SMs (a TMA box may have any number of rows;
 //     the lanes past R multiply whatever is in shared memory and are not read).  N = 28672: two slabs of 97 rows for each SM;
 //   * a CTA walks over its slabs; two accumulators in tensor memory, so that the epilogue of a slab overlaps the next one's loads;
-//   * where N is too small for that, K is split over the CTAs of a cluster.  Each keeps its int32 partial tile in tensor memory
-//     and, once all of its K is in, sends the rows of every 4 tokens to the CTA that owns them (group g: CTA g % split) through
-//     distributed shared memory.  Integer sums do not depend on the order, so results do not depend on the split, and nothing
-//     but D is written to global memory: calls on any number of streams and captured graphs share no scratch.
-//   warp 0 = TMA producer, warp 1 = MMA issuer + tensor-memory owner, warps 2..5 = exchange and epilogue.
+//   * warp 0 = TMA producer, warp 1 = MMA issuer + tensor-memory owner, warps 2..5 = epilogue.
+//
+// Short streams: an SM's share of the weights is a few dozen KB, and a single pass through TMA, barriers and tensor memory costs
+// more than the bytes.  A CTA takes 16 rows; its warps take 128-byte pieces of K in turn, straight from global memory into the
+// registers of warp-level MMAs (m16n8k32), all loads of a thread in flight together, and add up in shared memory.
 #include <atomic>
 #include "ptx.cuh"
 #include "internal.h"
@@ -19,11 +22,7 @@
 namespace tkb {
 
 constexpr int kSkinnyStages = 16;
-// Shared memory of a CTA.  Short streams of weights leave half an SM's, so that the next kernel's CTAs set themselves up, and ask L2
-// for their weights, while this kernel ends: M=32 N=2048 K=7168 6.6 us against 10.7 us with the large one, whose CTAs (clusters,
-// above all) only start once the SM is empty.  Long streams gain more from a deeper ring: M=16 N=28672 K=8192 38.9 us against 41.2.
-constexpr int kSkinnySmemShort = 112 * 1024, kSkinnySmemLong = 208 * 1024;
-constexpr int kSkinnyLongStream = 384 * 1024;       // bytes of weights of one CTA
+constexpr int kSkinnySmem = 208 * 1024;
 
 template <int NB>
 struct SkinnyCfg {
@@ -37,11 +36,9 @@ struct SkinnyCfg {
 struct SkinnyParams {
     const float* a_sc; const float* b_sc;
     void* D; int64_t ldd;
-    int M, N, kblk, out_dtype;
-    int rows, slabs, split_log2;            // weight rows of a slab, slabs, log2 of the CTAs that share a slab's K
+    int M, N, K, out_dtype;
+    int rows, slabs;                        // weight rows of a slab, slabs
     int stages, w_bytes;                    // operand ring: stages, bytes from one stage's weights to the next's
-    int prefetch;                           // K blocks of its weights that a CTA asks L2 for before the previous kernel is done
-    int smem;                               // bytes of dynamic shared memory
     int* status;
     long long wait_limit;
 };
@@ -55,11 +52,6 @@ __device__ __forceinline__ void tmem_ld_32x16_i(uint32_t taddr, uint32_t* r) {
         : "r"(taddr)
         : "memory");
 }
-
-// Cluster barrier of warps whose lanes may come out of a wait one after the other: the forms without .aligned, and the lanes
-// together first.
-__device__ __forceinline__ void split_arrive() { __syncwarp(); asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void split_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); __syncwarp(); }
 
 __device__ __forceinline__ void store_out(const SkinnyParams& p, int m, int n, int sum, float a_sc, float b_sc) {
     const float v = __int2float_rn(sum) * a_sc * b_sc;
@@ -83,14 +75,10 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int nst = p.stages;
-    const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sX = smem0;                                      // tokens first: an MMA reads 128 rows from a stage's weights on
-    const uint32_t sW = smem0 + nst * C::X_BYTES;
-    const uint32_t sRecv = smem0;                                   // split K: partial sums, once every ring of the cluster is idle
-    const int split = 1 << p.split_log2;
-    const int rank = split > 1 ? int(cluster_ctarank()) : 0;
-    const int unit = int(blockIdx.x) >> p.split_log2, units = int(gridDim.x) >> p.split_log2;
-    const int kb0 = (p.kblk * rank) >> p.split_log2, kb1 = (p.kblk * (rank + 1)) >> p.split_log2;
+    const uint32_t sX = (smem_u32(smem_raw) + 1023u) & ~1023u;      // tokens first: an MMA reads 128 rows from a stage's weights on
+    const uint32_t sW = sX + nst * C::X_BYTES;
+    const int unit = int(blockIdx.x), units = int(gridDim.x);
+    const int kblk = (p.K + 127) / 128;
 
     if (threadIdx.x == 0) {
         s_abort = 0;
@@ -110,19 +98,13 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     WaitCtx wc{&s_abort, p.status, p.wait_limit};
 
     if (warp == 0) {
-        const bool leader = elect_one();
-        uint32_t stage = 0, phase = 0, issued = 0;
-        bool ok = true;
-        if (leader) {
-            // Weights may be asked for before the previous kernel is done, whoever writes them: this only moves lines into L2,
-            // where a later write finds them.
-            int left = p.prefetch;
-            for (int slab = unit; slab < p.slabs && left > 0; slab += units)
-                for (int kb = kb0; kb < kb1 && left > 0; kb++, left--) tma_prefetch_2d(&tmW, kb * 128, slab * p.rows);
+        if (elect_one()) {
+            uint32_t stage = 0, phase = 0, issued = 0;
+            bool ok = true;
             asm volatile("griddepcontrol.wait;" ::: "memory");      // the tokens come from the kernel before this one
             const uint32_t tx = uint32_t(p.rows) * 128u + C::X_BYTES;
             for (int slab = unit; slab < p.slabs && ok; slab += units)
-                for (int kb = kb0; kb < kb1; kb++) {
+                for (int kb = 0; kb < kblk; kb++) {
                     if (!mbar_wait(wc, smem_u32(&bar_empty[stage]), phase ^ 1)) { ok = false; break; }
                     const uint32_t full = smem_u32(&bar_full[stage]);
                     mbar_arrive_expect_tx(full, tx);
@@ -131,12 +113,8 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                     issued++;
                     if (++stage == uint32_t(nst)) { stage = 0; phase ^= 1; }
                 }
-            // the memory system is about to run dry: let the next kernel set itself up and ask for its weights
+            // this SM's loads are all on their way: the next kernel may set itself up
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-        }
-        __syncwarp();
-        if (split > 1) split_arrive();      // (1): the epilogue warps arrive when this CTA's MMAs are done
-        if (leader) {
             for (int s = 0; s < nst && ok; s++) {                   // stage releases of the MMA thread may still be in flight
                 ok = mbar_wait(wc, smem_u32(&bar_empty[stage]), phase ^ 1);
                 if (++stage == uint32_t(nst)) { stage = 0; phase ^= 1; }
@@ -144,7 +122,6 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             if (!ok) drain_ring(bar_full, nst, issued, p.wait_limit);
         }
         __syncwarp();
-        if (split > 1) { split_wait(); split_arrive(); split_wait(); }
     } else if (warp == 1) {
         if (elect_one()) {
             uint32_t stage = 0, phase = 0, seg = 0;
@@ -153,14 +130,14 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 const uint32_t buf = seg & 1u;
                 if (!mbar_wait(wc, smem_u32(&bar_acc_empty[buf]), ((seg >> 1) & 1u) ^ 1u)) { ok = false; break; }
                 tc_fence_after();
-                for (int kb = kb0; kb < kb1; kb++) {
+                for (int kb = 0; kb < kblk; kb++) {
                     if (!mbar_wait(wc, smem_u32(&bar_full[stage]), phase)) { ok = false; break; }
                     tc_fence_after();
                     const uint64_t a_desc = smem_desc_sw128(sW + stage * p.w_bytes);
                     const uint64_t b_desc = smem_desc_sw128(sX + stage * C::X_BYTES);
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        mma_i8<1>(tmem_base + buf * C::ACC_COLS, a_desc + 2 * j, b_desc + 2 * j, idesc_int8(128, NB), (kb > kb0 || j > 0) ? 1u : 0u);
+                        mma_i8<1>(tmem_base + buf * C::ACC_COLS, a_desc + 2 * j, b_desc + 2 * j, idesc_int8(128, NB), (kb > 0 || j > 0) ? 1u : 0u);
                     tc_commit<1>(smem_u32(&bar_empty[stage]));
                     if (++stage == uint32_t(nst)) { stage = 0; phase ^= 1; }
                 }
@@ -168,89 +145,36 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             }
         }
         __syncwarp();
-        if (split > 1) { split_arrive(); split_wait(); split_arrive(); split_wait(); }
     } else {
         const int quarter = warp & 3;
         const int n_local = quarter * 32 + lane;
         asm volatile("griddepcontrol.wait;" ::: "memory");          // D may still be read, and the scales written, by the kernel before this one
-        if (split == 1) {
-            uint32_t seg = 0;
-            for (int slab = unit; slab < p.slabs; slab += units, seg++) {
-                const uint32_t buf = seg & 1u;
-                const int n = slab * p.rows + n_local;
-                const bool mine = n_local < p.rows && n < p.N;
-                const float b_sc = mine ? __ldg(p.b_sc + n) : 0.f;
-                const bool full = mbar_wait(wc, smem_u32(&bar_acc_full[buf]), (seg >> 1) & 1u);
-                if (!__all_sync(0xffffffffu, full)) break;          // (lanes together: the loads below are the warp's)
-                tc_fence_after();
-#pragma unroll
-                for (int c0 = 0; c0 < NB; c0 += C::CHUNK) {
-                    if (c0 < p.M) {
-                        uint32_t r[C::CHUNK];
-                        const uint32_t at = tmem_base + (uint32_t(quarter * 32) << 16) + buf * C::ACC_COLS + c0;
-                        if constexpr (C::CHUNK == 32) tmem_ld_32x32(at, r); else tmem_ld_32x16_i(at, r);
-                        tmem_ld_wait();
-                        if (mine) {
-#pragma unroll
-                            for (int i = 0; i < C::CHUNK; i++)
-                                if (c0 + i < p.M) store_out(p, c0 + i, n, int(r[i]), __ldg(p.a_sc + c0 + i), b_sc);
-                        }
-                    }
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&bar_acc_empty[buf]));
-            }
-        } else {
-            // one slab for each cluster (units >= slabs)
-            const int n = unit * p.rows + n_local;
+        uint32_t seg = 0;
+        for (int slab = unit; slab < p.slabs; slab += units, seg++) {
+            const uint32_t buf = seg & 1u;
+            const int n = slab * p.rows + n_local;
             const bool mine = n_local < p.rows && n < p.N;
             const float b_sc = mine ? __ldg(p.b_sc + n) : 0.f;
-            const bool ok = __all_sync(0xffffffffu, mbar_wait(wc, smem_u32(&bar_acc_full[0]), 0));
+            const bool full = mbar_wait(wc, smem_u32(&bar_acc_full[buf]), (seg >> 1) & 1u);
+            if (!__all_sync(0xffffffffu, full)) break;              // (lanes together: the loads below are the warp's)
             tc_fence_after();
-            split_arrive();                                         // (1)
-            split_wait();                                           // every CTA's MMAs are done: the rings may be written over
-            if (ok) {
 #pragma unroll
-                for (int c0 = 0; c0 < NB; c0 += C::CHUNK) {
-                    if (c0 < p.M) {
-                        uint32_t r[C::CHUNK];
-                        const uint32_t at = tmem_base + (uint32_t(quarter * 32) << 16) + c0;
-                        if constexpr (C::CHUNK == 32) tmem_ld_32x32(at, r); else tmem_ld_32x16_i(at, r);
-                        tmem_ld_wait();
-                        // tokens 4 g .. 4 g + 3 go to CTA g % split: [g / split][source CTA][weight row][4]
+            for (int c0 = 0; c0 < NB; c0 += C::CHUNK) {
+                if (c0 < p.M) {
+                    uint32_t r[C::CHUNK];
+                    const uint32_t at = tmem_base + (uint32_t(quarter * 32) << 16) + buf * C::ACC_COLS + c0;
+                    if constexpr (C::CHUNK == 32) tmem_ld_32x32(at, r); else tmem_ld_32x16_i(at, r);
+                    tmem_ld_wait();
+                    if (mine) {
 #pragma unroll
-                        for (int i = 0; i < C::CHUNK; i += 4) {
-                            const int g = (c0 + i) >> 2, owner = g & (split - 1);
-                            if (c0 + i < p.M) {
-                                const uint32_t dst = mapa(sRecv + uint32_t((g - owner + rank) * 128 + n_local) * 16, uint32_t(owner));
-                                asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]) : "memory");
-                            }
-                        }
+                        for (int i = 0; i < C::CHUNK; i++)
+                            if (c0 + i < p.M) store_out(p, c0 + i, n, int(r[i]), __ldg(p.a_sc + c0 + i), b_sc);
                     }
                 }
             }
             tc_fence_before();
-            split_arrive();                                         // (2)
-            split_wait();                                           // the partial sums sent above are where they belong
-            if (ok && mine) {
-                for (int g = rank; 4 * g < p.M; g += split) {
-                    const uint32_t src = sRecv + uint32_t((g - rank) * 128 + n_local) * 16;
-                    int sum[4] = {0, 0, 0, 0};
-#pragma unroll
-                    for (int s = 0; s < 8; s++) {
-                        if (s < split) {
-                            int v[4];
-                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src + s * 2048));
-#pragma unroll
-                            for (int i = 0; i < 4; i++) sum[i] += v[i];
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (4 * g + i < p.M) store_out(p, 4 * g + i, n, sum[i], __ldg(p.a_sc + 4 * g + i), b_sc);
-                }
-            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&bar_acc_empty[buf]));
         }
     }
     __syncthreads();
@@ -260,74 +184,173 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
 }
 
-// How N and K are cut.  Slabs of a CTA's share of N, in as few pieces of at most 128 rows as it takes, if that share is a fair
-// tile; else K is split, which keeps the tokens from being read by more CTAs than needed.  Cost of a 128-byte K block on a CTA in
-// cycles: its bytes at an SM's share of the HBM rate (23 bytes a cycle; tokens, from L2, at twice that), but not below the 420
-// that its barriers, copies and MMAs take to issue; an exchange of partial sums on top.  Measured, M=1 N=2048 K=7168: split 1 (14
-// rows, 56 blocks) 12.5 us, 2 9.2 us, 4 6.6 us, 8 5.7 us.
-static void skinny_plan(int M, int N, int K, int sm_count, int nb, SkinnyParams& p) {
-    const int kblk = (K + 127) / 128;
-    double best = 1e30;
-    for (int lg = 0; lg <= 3; lg++) {
-        const int split = 1 << lg;
-        if (split > kblk) break;
-        const int units = lg == 3 ? sm_count / 8 - 2 : (lg == 2 ? sm_count / 4 - 1 : sm_count / split);         // clusters that the GPCs hold at once
-        const int per_unit = ((N + 127) / 128 + units - 1) / units;                                             // slabs
-        if (lg > 0 && per_unit > 1) break;
-        const int rows = (N + units * per_unit - 1) / (units * per_unit);
-        const double block = (rows + 0.5 * M) * 128 / 23.0;
-        const double cost = double(per_unit) * ((kblk + split - 1) / split) * (block < 420 ? 420 : block) + (lg ? 1400 + 10 * M : 0);
-        if (cost < best) {
-            best = cost;
-            p.split_log2 = lg; p.rows = rows; p.slabs = (N + rows - 1) / rows;
-            p.smem = double(per_unit) * rows * K / split >= kSkinnyLongStream ? kSkinnySmemLong : kSkinnySmemShort;
+// ---- short streams --------------------------------------------------------------------------
+
+// 16 bytes at p, of which the first `left` belong to the row; the others count as zeros.  TAIL: rows may end inside 16 bytes.
+template <bool TAIL>
+__device__ __forceinline__ uint4 load16(const uint8_t* p, int left) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (left >= (TAIL ? 16 : 1)) v = __ldg(reinterpret_cast<const uint4*>(p));
+    if constexpr (TAIL) {
+        if (left > 0 && left < 16) {
+            uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < 15; i++)
+                if (i < left) w[i >> 2] |= uint32_t(__ldg(p + i)) << (8 * (i & 3));
+            v = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
-    p.kblk = kblk;
-    p.w_bytes = (p.rows * 128 + 1023) / 1024 * 1024;
-    p.stages = (p.smem - 1024 - (128 * 128 - p.w_bytes)) / (p.w_bytes + nb * 128);       // the last stage's MMAs read 128 rows
-    if (p.stages > kSkinnyStages) p.stages = kSkinnyStages;
-    p.prefetch = (p.smem == kSkinnySmemLong ? 256 : 64) * 1024 / (p.rows * 128);
+    return v;
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <int NB>
-static cudaError_t launch_skinny_t(const SkinnyArgs& a, const SkinnyParams& p) {
-    using C = SkinnyCfg<NB>;
-    auto kern = int8_skinny_kernel<NB>;
+constexpr int kShortWarps = 16;
+constexpr int kShortRows = 16;
+
+struct ShortParams {
+    SkinnyParams s;
+    const uint8_t* A; const uint8_t* B;
+    int64_t lda, ldb;
+};
+
+// One CTA: weight rows 16 blockIdx.x .. + 15 (the MMA's 16 rows) times tokens 8 TT blockIdx.y .. + 8 TT - 1 (its columns).  In a piece of 128 bytes of K,
+// lane 4 g + t holds bytes 16 t .. 16 t + 15 of each half, of rows g and g + 8 and of token g: the words of a 16-byte load are the
+// operands of two MMAs.  That assigns the bytes of K to the MMA's K indices in another order than memory's, but to both operands
+// alike, which a sum does not notice.
+template <int TT, bool TAIL>
+__global__ void __launch_bounds__(kShortWarps * 32) int8_short_kernel(const ShortParams q) {
+    const SkinnyParams& p = q.s;
+    const int m0 = int(blockIdx.y) * 8 * TT, M = p.M - m0;
+    const uint8_t* A = q.A + int64_t(m0) * q.lda;
+    extern __shared__ int red[];                                    // [warp][16 rows][8 TT tokens]
+    constexpr int TOKENS = 8 * TT;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = int(blockIdx.x) * kShortRows;
+    const uint8_t* w0 = n0 + g < p.N ? q.B + int64_t(n0 + g) * q.ldb : nullptr;
+    const uint8_t* w1 = n0 + g + 8 < p.N ? q.B + int64_t(n0 + g + 8) * q.ldb : nullptr;
+    int acc[TT][4] = {};
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    constexpr int UNROLL = TT <= 2 ? 4 : 2;
+    for (int k0 = warp * 128; k0 < p.K; k0 += kShortWarps * 128 * UNROLL) {
+        uint4 a[UNROLL][2][2];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = k0 + u * kShortWarps * 128 + h * 64 + t * 16;
+                a[u][h][0] = load16<TAIL>(w0 + k, w0 ? p.K - k : 0);
+                a[u][h][1] = load16<TAIL>(w1 + k, w1 ? p.K - k : 0);
+            }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = k0 + u * kShortWarps * 128 + h * 64 + t * 16;
+                uint4 b[TT];
+#pragma unroll
+                for (int c = 0; c < TT; c++) b[c] = load16<TAIL>(A + int64_t(8 * c + g) * q.lda + k, 8 * c + g < M ? p.K - k : 0);
+#pragma unroll
+                for (int c = 0; c < TT; c++) {
+                    mma_s8(acc[c], a[u][h][0].x, a[u][h][1].x, a[u][h][0].y, a[u][h][1].y, b[c].x, b[c].y);
+                    mma_s8(acc[c], a[u][h][0].z, a[u][h][1].z, a[u][h][0].w, a[u][h][1].w, b[c].z, b[c].w);
+                }
+            }
+    }
+    // result i of tile c: row g + 8 (i / 2), token 8 c + 2 t + i % 2
+#pragma unroll
+    for (int c = 0; c < TT; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) red[(warp * TOKENS + 8 * c + 2 * t + (i & 1)) * kShortRows + g + 8 * (i >> 1)] = acc[c][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < TOKENS * kShortRows; e += kShortWarps * 32) {
+        const int m = e / kShortRows, n = n0 + e % kShortRows;
+        if (m >= M || n >= p.N) continue;
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < kShortWarps; w++) sum += red[w * TOKENS * kShortRows + e];
+        store_out(p, m0 + m, n, sum, __ldg(p.a_sc + m0 + m), __ldg(p.b_sc + n));
+    }
+}
+
+// ---- launches -------------------------------------------------------------------------------
+
+static cudaError_t launch_dependent(const void* kern, dim3 grid, int threads, int smem, cudaStream_t stream, void** args, int smem_attr, std::atomic<bool>* attr_set) {
     // the attribute belongs to the (kernel, device) pair: remember it per device, not per process
-    static std::atomic<bool> attr_set[64] = {};
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
-        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkinnySmemLong); e != cudaSuccess) return e;
+        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_attr); e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) attr_set[dev].store(true, std::memory_order_release);
     }
-    const int split = 1 << p.split_log2;
-    const int units = split > 1 || p.slabs < a.sm_count ? p.slabs : a.sm_count;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(units) * split); cfg.blockDim = dim3(C::THREADS); cfg.dynamicSmemBytes = p.smem; cfg.stream = a.stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kern, a.tmW, a.tmX, p);
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelExC(&cfg, kern, args);
+}
+
+// Slabs: every SM's share of N, in as few pieces of at most 128 rows as it takes.
+static void skinny_plan(int N, int sm_count, int nb, SkinnyParams& p) {
+    const int per_sm = ((N + 127) / 128 + sm_count - 1) / sm_count;
+    p.rows = (N + sm_count * per_sm - 1) / (sm_count * per_sm);
+    p.slabs = (N + p.rows - 1) / p.rows;
+    p.w_bytes = (p.rows * 128 + 1023) / 1024 * 1024;
+    p.stages = (kSkinnySmem - 1024 - (128 * 128 - p.w_bytes)) / (p.w_bytes + nb * 128);       // the last stage's MMAs read 128 rows
+    if (p.stages > kSkinnyStages) p.stages = kSkinnyStages;
+}
+
+template <int NB>
+static cudaError_t launch_skinny_t(const SkinnyArgs& a, SkinnyParams p) {
+    static std::atomic<bool> attr_set[64] = {};
+    CUtensorMap tmW = a.tmW, tmX = a.tmX;
+    void* args[3] = {&tmW, &tmX, &p};
+    return launch_dependent(reinterpret_cast<const void*>(int8_skinny_kernel<NB>), dim3(unsigned(p.slabs < a.sm_count ? p.slabs : a.sm_count)), SkinnyCfg<NB>::THREADS,
+                            kSkinnySmem, a.stream, args, kSkinnySmem, attr_set);
+}
+
+template <int TT, bool TAIL>
+static cudaError_t launch_short_t(const SkinnyArgs& a, const SkinnyParams& p) {
+    static std::atomic<bool> attr_set[64] = {};
+    ShortParams q{p, static_cast<const uint8_t*>(a.A), static_cast<const uint8_t*>(a.B), a.lda, a.ldb};
+    void* args[1] = {&q};
+    constexpr int smem = kShortWarps * kShortRows * 8 * TT * 4;
+    return launch_dependent(reinterpret_cast<const void*>(int8_short_kernel<TT, TAIL>), dim3(unsigned((p.N + kShortRows - 1) / kShortRows), unsigned((p.M + 8 * TT - 1) / (8 * TT))), kShortWarps * 32, smem,
+                            a.stream, args, smem, attr_set);
+}
+template <bool TAIL>
+static cudaError_t launch_short(const SkinnyArgs& a, const SkinnyParams& p) {
+    if (a.M <= 8) return launch_short_t<1, TAIL>(a, p);
+    if (a.M <= 16) return launch_short_t<2, TAIL>(a, p);
+    if (a.M <= 32) return launch_short_t<4, TAIL>(a, p);
+    return launch_short_t<8, TAIL>(a, p);
 }
 
 int int8_skinny_padded_rows(int M) { return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)); }
-int int8_skinny_slab_rows(int M, int N, int K, int sm_count) {
+int int8_skinny_slab_rows(int M, int N, int sm_count) {
     SkinnyParams p;
-    skinny_plan(M, N, K, sm_count, int8_skinny_padded_rows(M), p);
+    skinny_plan(N, sm_count, int8_skinny_padded_rows(M), p);
     return p.rows;
 }
+// Long streams pay about 0.2 us for each 128-byte block of K, however few weight rows an SM has; short ones read the tokens again for
+// every 16 rows.  Measured, long / short in us: M=1 N=2048 K=7168 12.7 / 5.7, M=32 14.6 / 9.5, M=128 23.3 / 22.7; M=8 N=K=4096 8.9 / 5.9,
+// M=32 10.5 / 11.2; M=4 N=7168 K=2048 6.3 / 7.6; M=16 N=K=8192 16.2 / 19.6.
+bool int8_skinny_short(int M, int N, int sm_count) { return N <= (M <= 16 ? 32 : 16) * sm_count; }
 
 cudaError_t launch_int8_skinny(const SkinnyArgs& a) {
     SkinnyParams p = {};
-    p.a_sc = a.a_sc; p.b_sc = a.b_sc; p.D = a.D; p.ldd = a.ldd; p.M = a.M; p.N = a.N; p.out_dtype = a.out_dtype;
+    p.a_sc = a.a_sc; p.b_sc = a.b_sc; p.D = a.D; p.ldd = a.ldd; p.M = a.M; p.N = a.N; p.K = a.K; p.out_dtype = a.out_dtype;
     p.status = a.status; p.wait_limit = api_wait_limit();
+    if (int8_skinny_short(a.M, a.N, a.sm_count)) {
+        return a.K % 16 ? launch_short<true>(a, p) : launch_short<false>(a, p);
+    }
     const int nb = int8_skinny_padded_rows(a.M);
-    skinny_plan(a.M, a.N, a.K, a.sm_count, nb, p);
+    skinny_plan(a.N, a.sm_count, nb, p);
     switch (nb) {
         case 16: return launch_skinny_t<16>(a, p);
         case 32: return launch_skinny_t<32>(a, p);

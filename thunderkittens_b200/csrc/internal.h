@@ -57,7 +57,8 @@ struct MoeParams {
     unsigned int epoch;
     int rank, world, comm_ctas, expert_rows; // expert_rows = rows of one expert's weight matrix (the GEMM's N)
 };
-enum GemmMode : int { MODE_PLAIN = 0, MODE_AG = 1, MODE_MOE = 2, MODE_QUANT = 4, MODE_RS = 8 };   // QUANT: the epilogue writes D as NVFP4; RS: reduce-scatter
+enum GemmMode : int { MODE_PLAIN = 0, MODE_AG = 1, MODE_MOE = 2, MODE_QUANT = 4, MODE_RS = 8,   // QUANT: the epilogue writes D as NVFP4; RS: reduce-scatter
+                      MODE_DIRECT = 16 };                                                                // KIND_INT8: D is stored without TMA
 struct CommParams { AgParams ag; MoeParams moe; };
 
 struct GemmArgs {
@@ -77,9 +78,9 @@ struct GemmArgs {
     // MODE_RS: the bf16 tiles are reduce-added into the output of the rank that owns their rows.  rs_maps: `rs_world` tensor maps in
     // DEVICE memory, map i over rank i's output [M / world, N] bf16 (box 64 x 32, 128-byte swizzle, as tmD); rs_rank rotates the tile order
     const CUtensorMap* rs_maps; int rs_rows_per_rank, rs_rank, rs_world;
-    // KIND_INT8: sgA / sgB hold one scale per row; D has out_dtype (TKB_DTYPE_*).  With plain_out D is stored without TMA (its base
-    // or pitch is not a multiple of 16 bytes) from these two
-    int out_dtype, plain_out;
+    // KIND_INT8: sgA / sgB hold one scale per row; D has out_dtype (TKB_DTYPE_*).  MODE_DIRECT stores it without TMA (its base or
+    // pitch is not a multiple of 16 bytes) at these two
+    int out_dtype;
     void* D; int64_t ldd;
 };
 cudaError_t launch_gemm(const GemmArgs& a);
@@ -105,7 +106,8 @@ int decode_padded_rows(int M);
 // int8_skinny.cu
 constexpr int kInt8SkinnyMaxM = 128;
 struct SkinnyArgs {
-    CUtensorMap tmW, tmX;       // boxes of 128 bytes of K x int8_skinny_slab_rows() weight rows / int8_skinny_padded_rows() tokens, 128-byte swizzle
+    CUtensorMap tmW, tmX;       // long streams: boxes of 128 bytes of K x int8_skinny_slab_rows() weight rows / int8_skinny_padded_rows() tokens, 128-byte swizzle
+    const void* A; int64_t lda; const void* B; int64_t ldb;
     const float* a_sc; const float* b_sc;
     void* D; int64_t ldd;
     int M, N, K, out_dtype;
@@ -113,6 +115,7 @@ struct SkinnyArgs {
 };
 cudaError_t launch_int8_skinny(const SkinnyArgs& a);
 int int8_skinny_padded_rows(int M);
-int int8_skinny_slab_rows(int M, int N, int K, int sm_count);
+int int8_skinny_slab_rows(int M, int N, int sm_count);
+bool int8_skinny_short(int M, int N, int sm_count);     // short streams: no tensor maps
 
 } // namespace tkb

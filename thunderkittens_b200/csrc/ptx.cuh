@@ -144,10 +144,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* map, uint3
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
-// The same tile into L2 only.
-__device__ __forceinline__ void tma_prefetch_2d(const void* map, int x, int y) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y) : "memory");
-}
 // 2-D tiled load into this CTA's shared memory whose completion bytes are credited to an mbarrier
 // that may live in the peer CTA of a CTA pair (bar is a shared::cluster address).  No multicast.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* map, uint32_t cluster_bar, int x, int y) {
