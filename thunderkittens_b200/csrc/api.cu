@@ -364,7 +364,10 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
     memset(&g, 0, sizeof(g));
     g.kind = KIND_INT8;
     g.config = pick_config(KIND_INT8, config, M, N, c->sm_count);
-    // one wave of 128 x 128 tiles rather than two of CTA pairs: M=333 N=5000 K=4112 17.9 us against 24.1 us
+    // short K: the epilogue counts for more than the loads that a CTA pair saves (M=N=8192, pairs / single CTAs: K=512 48.6 / 41.8 us, K=1024
+    // 60.4 / 60.5 us, K=2048 94.2 / 103.5 us)
+    if (config == TKB_GEMM_DEFAULT && K < 1024) g.config |= 1;
+    // one wave of 128 x 128 tiles rather than two of CTA pairs: M=333 N=5000 K=4112 17.9 us against 24.0 us
     if (config == TKB_GEMM_DEFAULT && g.config == 2 && long((M + 255) / 256) * ((N + 127) / 128) * 2 > c->sm_count &&
         long((M + 127) / 128) * ((N + 127) / 128) <= c->sm_count)
         g.config = 3;

@@ -59,7 +59,7 @@ struct GemmCfg {
     static constexpr int SFA_BYTES = SF_CHUNKS * 512;
     static constexpr int SFB_BYTES = SF_CHUNKS * 512 * (BN / 128);
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
-    static constexpr int EPI_WARPS = BN == 256 ? 8 : 4;
+    static constexpr int EPI_WARPS = BN == 256 || KIND == KIND_INT8 ? 8 : 4;
     static constexpr int EPI_WARP_BYTES = 32 * 128;                  // one 32-row x 64-column bf16 store box per warp
     static constexpr int EPI_BYTES = EPI_WARPS * EPI_WARP_BYTES;
     static constexpr int SMEM_BUDGET = 227 * 1024 - 2048 - EPI_BYTES;
@@ -828,7 +828,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 const int col0 = n_blk * BN + col_base;
                 const uint32_t acc_t = tmem_base + (uint32_t(quarter * 32) << 16) + buf * C::ACC_COLS + col_base;
                 int8_epilogue<MODE == MODE_DIRECT>(acc_t, &tmD, p, stage_box, row0, col0, row_scale, lane, d_policy);
-                int8_epilogue<MODE == MODE_DIRECT>(acc_t + 64, &tmD, p, stage_box, row0, col0 + 64, row_scale, lane, d_policy);
+                if (C::COLS_PER_EPI_WARP > 64)
+                    int8_epilogue<MODE == MODE_DIRECT>(acc_t + 64, &tmD, p, stage_box, row0, col0 + 64, row_scale, lane, d_policy);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {                             // (two accumulators: the next tile's MMAs are under way)
