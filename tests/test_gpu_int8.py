@@ -244,6 +244,26 @@ def test_linear_on_two_streams_and_in_graphs(cuda, lib, M):
         layer.check()
 
 
+@pytest.mark.parametrize("M", [2, 30, 100, 260])
+def test_linear_with_operands_that_change_every_call(cuda, lib, M):
+    """Launches that begin while the ones before them end read what those wrote: the same buffers, other values, no waiting."""
+    ops, N, K, R = _ops(), 700, 1024, 24
+    g = torch.Generator(device=cuda).manual_seed(M)
+    xs = torch.randn(R, M, K, generator=g, device=cuda).to(torch.bfloat16) * (1 + torch.arange(R, device=cuda).to(torch.bfloat16))[:, None, None]
+    w = torch.randn(R, N, K, generator=g, device=cuda).to(torch.bfloat16)
+    q, sc, b, b_sc = torch.empty(M, K, dtype=torch.int8, device=cuda), torch.empty(M, device=cuda), torch.empty(N, K, dtype=torch.int8, device=cuda), torch.empty(N, device=cuda)
+    Ds = torch.empty(R, M, N, device=cuda)
+    torch.cuda.synchronize()
+    for i in range(R):
+        ops.int8_quantize(w[i], b, b_sc)
+        ops.int8_quantize(xs[i], q, sc)
+        ops.int8_gemm(q, sc, b, b_sc, Ds[i])
+    for i in range(R):
+        codes, steps = quantize64(xs[i])
+        w_codes, w_steps = quantize64(w[i])
+        _check_gemm(Ds[i], codes, steps.float(), w_codes, w_steps.float())
+
+
 def test_refusals_on_tensors(cuda, lib):
     ops = _ops()
     a, a_sc, b, b_sc = _operands(20, 32, 64, cuda)

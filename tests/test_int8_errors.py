@@ -20,6 +20,8 @@ def test_int8_quantize(lib):
     assert f(None, 0, BF16, Q, 0, S, 4, 64, None) == INVALID and "null" in _msg(lib)
     assert f(A, 0, BF16, None, 0, S, 4, 64, None) == INVALID and f(A, 0, BF16, Q, 0, None, 4, 64, None) == INVALID
     assert f(A, 0, FP32, Q, 0, S, 4, 64, None) == INVALID and "dtype" in _msg(lib)
+    assert f(A, 0, BF16, Q, 0, A + 256, 4, 64, None) == INVALID and f(A, 0, BF16, Q, 0, Q + 252, 4, 64, None) == INVALID and "overlap" in _msg(lib)
+    assert f(A, 0, BF16, Q, 0, S, 2 ** 30 + 1, 64, None) == INVALID
     assert f(A, 0, BF16, Q, 0, S, -1, 64, None) == INVALID and f(A, 0, BF16, Q, 0, S, 4, 0, None) == INVALID
     assert f(A, 0, BF16, Q, 0, S, 4, 65537, None) == INVALID and "65536" in _msg(lib)
     assert f(A, 63, BF16, Q, 0, S, 4, 64, None) == ALIGN and f(A, 0, BF16, Q, 63, S, 4, 64, None) == ALIGN
@@ -38,7 +40,7 @@ def test_int8_gemm(lib):
         args[i] = None
         assert f(*args) == INVALID and "null" in _msg(lib)
     assert f(A, 0, SA, B, 0, SB, D, 0, 3, 8, 8, 64, None) == INVALID and "dtype" in _msg(lib)
-    for M, N, K in ((-1, 8, 64), (8, 0, 64), (8, 8, 0), (8, 8, 131072)):
+    for M, N, K in ((-1, 8, 64), (8, 0, 64), (8, 8, 0), (2 ** 30 + 1, 8, 64), (8, 2 ** 31 - 1, 64), (8, 8, 131072)):
         assert f(A, 0, SA, B, 0, SB, D, 0, BF16, M, N, K, None) == INVALID
     assert "131071" in _msg(lib)
     assert f(A, 0, SA, B, 0, SB, D, 0, BF16, 8, 8, 72, None) == ALIGN and "padded" in _msg(lib)
@@ -78,6 +80,8 @@ def test_block_norm(lib):
     assert call(per=0) == INVALID and "rows_per_gate" in _msg(lib)
     assert call(dtype=FP32) == INVALID and call(K=16385) == INVALID and call(q=Q) == INVALID
     assert call(r=H) == INVALID and call(r=X, ldr=128) == INVALID and call(r=X + 2) == INVALID and call(y=X) == INVALID and call(y=R) == INVALID and "overlap" in _msg(lib)
+    assert call(y=V) == INVALID and call(r=W) == INVALID and call(y=G + 126) == INVALID and call(y=G - 510, per=1) == INVALID and "gate" in _msg(lib)
+    assert call(rs=float("inf")) == INVALID and call(rs=float("nan")) == INVALID and "residual_scale" in _msg(lib)
     assert call(gate=G + 1) == ALIGN and call(ldg=63) == ALIGN and call(ldr=1) == ALIGN
     assert call(h=None, x=None, r=None, w_post=None, gate=None, w_pre=None, y=None, M=0) == 0
 

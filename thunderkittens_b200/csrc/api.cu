@@ -327,7 +327,8 @@ static int gemm_common(int kind, const void* A, int64_t lda_bytes, const void* A
 static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const void* B, int64_t ldb, const float* B_sc, void* D, int64_t ldd, int dtype,
                             int M, int N, int K, int config, void* stream) {
     if (dtype != TKB_DTYPE_BF16 && dtype != TKB_DTYPE_FP16 && dtype != TKB_DTYPE_FP32) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: unknown output dtype %d", dtype);
-    if (M < 0 || N < 1 || K < 1) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: need M >= 0 and N, K >= 1 (got %d, %d, %d)", M, N, K);
+    if (M < 0 || N < 1 || K < 1 || M > (1 << 30) || N > (1 << 30))
+        return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: need M >= 0, N, K >= 1 and M, N <= 2^30 (got %d, %d, %d)", M, N, K);
     if (K > kInt8MaxK) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: K=%d is above %d, where a sum of K products may leave int32", K, kInt8MaxK);
     if (config < TKB_GEMM_DEFAULT || config > TKB_GEMM_SINGLE_N128) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: config %d is not a tile of this format", config);
     if (lda == 0) lda = K;

@@ -192,7 +192,7 @@ __device__ __forceinline__ void int8_epilogue(uint32_t acc_t, const CUtensorMap*
         if (col + 32 <= p.N && (reinterpret_cast<uintptr_t>(cs) & 15u) == 0) {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float4 c = __ldg(reinterpret_cast<const float4*>(cs) + i);      // the same address in all lanes
+                const float4 c = reinterpret_cast<const float4*>(cs)[i];      // the same address in all lanes
                 r[4 * i] = __float_as_uint(__int2float_rn(int(r[4 * i])) * row_scale * c.x);
                 r[4 * i + 1] = __float_as_uint(__int2float_rn(int(r[4 * i + 1])) * row_scale * c.y);
                 r[4 * i + 2] = __float_as_uint(__int2float_rn(int(r[4 * i + 2])) * row_scale * c.z);
@@ -200,7 +200,7 @@ __device__ __forceinline__ void int8_epilogue(uint32_t acc_t, const CUtensorMap*
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__int2float_rn(int(r[i])) * row_scale * __ldg(p.sgB + min(col + i, p.N - 1)));
+            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__int2float_rn(int(r[i])) * row_scale * p.sgB[min(col + i, p.N - 1)]);
         }
         if (fp32) {
             box_free();
@@ -813,7 +813,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             float row_scale = 0.f;       // (a row that TMA clips or the plain stores leave out)
             if constexpr (KIND == KIND_INT8) {
                 const int row = m_blk * C::BM + int(cta_rank) * 128 + quarter * 32 + lane;
-                if (row < p.M) row_scale = __ldg(p.sgA + row);
+                if (row < p.M) row_scale = p.sgA[row];
             }
             (void)row_scale;
             const long long t0 = clock64();

@@ -162,7 +162,7 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             const uint32_t buf = seg & 1u;
             const int n = slab * p.rows + n_local;
             const bool mine = n_local < p.rows && n < p.N;
-            const float b_sc = mine ? __ldg(p.b_sc + n) : 0.f;
+            const float b_sc = mine ? p.b_sc[n] : 0.f;
             const bool full = mbar_wait(wc, smem_u32(&bar_acc_full[buf]), (seg >> 1) & 1u);
             if (!__all_sync(0xffffffffu, full)) break;              // (lanes together: the loads below are the warp's)
             tc_fence_after();
@@ -176,7 +176,7 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                     if (mine) {
 #pragma unroll
                         for (int i = 0; i < C::CHUNK; i++)
-                            if (c0 + i < p.M) store_out(p, c0 + i, n, int(r[i]), __ldg(p.a_sc + c0 + i), b_sc);
+                            if (c0 + i < p.M) store_out(p, c0 + i, n, int(r[i]), p.a_sc[c0 + i], b_sc);
                     }
                 }
             }
@@ -194,17 +194,19 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
 
 // ---- short streams --------------------------------------------------------------------------
 
+// (Plain loads here and below: what the kernel before this one wrote may not be read through the read-only path, which is free to
+// fetch before griddepcontrol.wait.)
 // 16 bytes at p, of which the first `left` belong to the row; the others count as zeros.  TAIL: rows may end inside 16 bytes.
 template <bool TAIL>
 __device__ __forceinline__ uint4 load16(const uint8_t* p, int left) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (left >= (TAIL ? 16 : 1)) v = __ldg(reinterpret_cast<const uint4*>(p));
+    if (left >= (TAIL ? 16 : 1)) v = *reinterpret_cast<const uint4*>(p);
     if constexpr (TAIL) {
         if (left > 0 && left < 16) {
             uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
             for (int i = 0; i < 15; i++)
-                if (i < left) w[i >> 2] |= uint32_t(__ldg(p + i)) << (8 * (i & 3));
+                if (i < left) w[i >> 2] |= uint32_t(p[i]) << (8 * (i & 3));
             v = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
@@ -223,15 +225,13 @@ struct ShortParams {
     const uint8_t* A; int64_t lda;
 };
 
-// One CTA: weight rows 16 blockIdx.x .. + 15 (the MMA's 16 rows) times tokens 8 TT blockIdx.y .. + 8 TT - 1 (its columns).  In a piece of 128 bytes of K,
+// One CTA: weight rows 16 blockIdx.x .. + 15 (the MMA's 16 rows) times up to 8 TT tokens (its columns).  In a piece of 128 bytes of K,
 // lane 4 g + t holds bytes 16 t .. 16 t + 15 of each half, of rows g and g + 8 and of token g: the words of a 16-byte load are the
 // operands of two MMAs.  That assigns the bytes of K to the MMA's K indices in another order than memory's, but to both operands
 // alike, which a sum does not notice.
 template <int TT, bool TAIL>
 __global__ void __launch_bounds__(kShortWarps * 32) int8_short_kernel(const ShortParams q) {
     const SkinnyParams& p = q.s;
-    const int m0 = int(blockIdx.y) * 8 * TT, M = p.M - m0;
-    const uint8_t* A = q.A + int64_t(m0) * q.lda;
     extern __shared__ int red[];                                    // [warp][16 rows][8 TT tokens]
     constexpr int TOKENS = 8 * TT;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) int8_short_kernel(const Shor
                 const int k = k0 + u * kShortWarps * 128 + h * 64 + t * 16;
                 uint4 b[TT];
 #pragma unroll
-                for (int c = 0; c < TT; c++) b[c] = load16<TAIL>(A + int64_t(8 * c + g) * q.lda + k, 8 * c + g < M ? p.K - k : 0);
+                for (int c = 0; c < TT; c++) b[c] = load16<TAIL>(q.A + int64_t(8 * c + g) * q.lda + k, 8 * c + g < p.M ? p.K - k : 0);
 #pragma unroll
                 for (int c = 0; c < TT; c++) {
                     mma_s8(acc[c], a[u][h][0].x, a[u][h][1].x, a[u][h][0].y, a[u][h][1].y, b[c].x, b[c].y);
@@ -275,11 +275,11 @@ __global__ void __launch_bounds__(kShortWarps * 32) int8_short_kernel(const Shor
     __syncthreads();
     for (int e = threadIdx.x; e < TOKENS * kShortRows; e += kShortWarps * 32) {
         const int m = e / kShortRows, n = n0 + e % kShortRows;
-        if (m >= M || n >= p.N) continue;
+        if (m >= p.M || n >= p.N) continue;
         int sum = 0;
 #pragma unroll
         for (int w = 0; w < kShortWarps; w++) sum += red[w * TOKENS * kShortRows + e];
-        store_out(p, m0 + m, n, sum, __ldg(p.a_sc + m0 + m), __ldg(p.b_sc + n));
+        store_out(p, m, n, sum, p.a_sc[m], p.b_sc[n]);
     }
 }
 
@@ -329,15 +329,14 @@ static cudaError_t launch_short_t(const SkinnyArgs& a, const SkinnyParams& p) {
     ShortParams q{p, static_cast<const uint8_t*>(a.A), a.lda};
     void* args[1] = {&q};
     constexpr int smem = kShortWarps * kShortRows * 8 * TT * 4;
-    return launch_dependent(reinterpret_cast<const void*>(int8_short_kernel<TT, TAIL>), dim3(unsigned((p.N + kShortRows - 1) / kShortRows), unsigned((p.M + 8 * TT - 1) / (8 * TT))), kShortWarps * 32, smem,
+    return launch_dependent(reinterpret_cast<const void*>(int8_short_kernel<TT, TAIL>), dim3(unsigned((p.N + kShortRows - 1) / kShortRows)), kShortWarps * 32, smem,
                             a.stream, args, smem, attr_set);
 }
 template <bool TAIL>
 static cudaError_t launch_short(const SkinnyArgs& a, const SkinnyParams& p) {
     if (a.M <= 8) return launch_short_t<1, TAIL>(a, p);
     if (a.M <= 16) return launch_short_t<2, TAIL>(a, p);
-    if (a.M <= 32) return launch_short_t<4, TAIL>(a, p);
-    return launch_short_t<8, TAIL>(a, p);
+    return launch_short_t<4, TAIL>(a, p);
 }
 
 int int8_skinny_padded_rows(int M) { return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)); }
@@ -347,9 +346,9 @@ int int8_skinny_slab_rows(int M, int N, int sm_count) {
     return p.rows;
 }
 // Long streams pay about 0.2 us for each 128-byte block of K, however few weight rows an SM has; short ones read the tokens again for
-// every 16 rows.  Measured, long / short in us: M=1 N=2048 K=7168 12.7 / 5.7, M=32 14.6 / 9.5, M=128 23.3 / 22.7; M=8 N=K=4096 8.9 / 5.9,
+// every 16 rows.  Measured, long / short in us: M=1 N=2048 K=7168 12.7 / 5.7, M=32 14.6 / 9.5, M=64 17.6 / 18.8; M=8 N=K=4096 8.9 / 5.9,
 // M=32 10.5 / 11.2; M=4 N=7168 K=2048 6.3 / 7.6; M=16 N=K=8192 16.2 / 19.6.
-bool int8_skinny_short(int M, int N, int sm_count) { return N <= (M <= 16 ? 32 : 16) * sm_count; }
+bool int8_skinny_short(int M, int N, int sm_count) { return M <= 32 && N <= (M <= 16 ? 32 : 16) * sm_count; }
 
 cudaError_t launch_int8_skinny(const SkinnyArgs& a) {
     SkinnyParams p = {};

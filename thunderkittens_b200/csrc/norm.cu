@@ -33,7 +33,7 @@ enum RowsKind : int { ROWS_WHOLE = 0, ROWS_SHIFTED = 1, ROWS_SINGLE = 2 };
 // How rows share a CTA: one row each (everything that depends on the row is uniform over the CTA); a row for each warp (no barriers);
 // several groups of warps with a row each, which also share weights in shared memory
 enum RowsLayout : int { ROWS_ONE = 0, ROWS_WARPS = 1, ROWS_STAGED = 2 };
-constexpr int kNormMaxK = 16384, kQuantMaxK = 65536;
+constexpr int kNormMaxK = 16384, kQuantMaxK = 65536, kMaxRows = 1 << 30;
 
 struct RowsParams {
     const void *x, *h, *w_post, *gate, *w_pre;
@@ -139,10 +139,10 @@ struct Slots {
         const uint16_t* v = static_cast<const uint16_t*>(vec);
         const int e = at(8 * g, shift);
         if constexpr (KIND == ROWS_WHOLE) {
-            if (e < K) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "l"(v + e));
+            if (e < K) asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "l"(v + e));
         } else if (KIND == ROWS_SHIFTED && e >= 0 && e + 8 <= K) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) b[i] = __ldg(v + e + 2 * i) | uint32_t(__ldg(v + e + 2 * i + 1)) << 16;
+            for (int i = 0; i < 4; i++) b[i] = v[e + 2 * i] | uint32_t(v[e + 2 * i + 1]) << 16;
         } else {
             gather(v, K, shift, g, b);
         }
@@ -489,21 +489,21 @@ static cudaError_t launch_rows_t(const RowsParams& p, int kind, int sm_count, cu
 }
 
 // ---- argument checks ------------------------------------------------------------------------
-struct Span { const char* name; const void* ptr; int64_t pitch, width; };     // bytes; M rows
+struct Span { const char* name; const void* ptr; int64_t rows, pitch, width; };     // pitch, width in bytes
 
 // Whether two row-strided buffers share a byte.  Column slices of one buffer (equal pitches) interleave without touching.
-static bool overlap(const Span& a, const Span& b, int M) {
+static bool overlap(const Span& a, const Span& b) {
     if (!a.ptr || !b.ptr) return false;
     const uintptr_t pa = reinterpret_cast<uintptr_t>(a.ptr), pb = reinterpret_cast<uintptr_t>(b.ptr);
-    if (pa + uintptr_t((M - 1) * a.pitch + a.width) <= pb || pb + uintptr_t((M - 1) * b.pitch + b.width) <= pa) return false;
-    if (a.pitch != b.pitch || M == 1) return true;
+    if (pa + uintptr_t((a.rows - 1) * a.pitch + a.width) <= pb || pb + uintptr_t((b.rows - 1) * b.pitch + b.width) <= pa) return false;
+    if (a.pitch != b.pitch || a.rows == 1 || b.rows == 1) return true;
     const int64_t d = pb >= pa ? int64_t((pb - pa) % uintptr_t(a.pitch)) : a.pitch - 1 - int64_t((pa - pb - 1) % uintptr_t(a.pitch));      // (pb - pa) mod pitch
     return d < a.width || d + b.width > a.pitch;
 }
 
 static int rows_call(const char* what, RowsParams p, int mode, int dtype, void* stream) {
     if (dtype != TKB_DTYPE_BF16 && dtype != TKB_DTYPE_FP16) return api_fail(TKB_ERR_INVALID_ARG, "%s: dtype %d is neither TKB_DTYPE_BF16 nor TKB_DTYPE_FP16", what, dtype);
-    if (p.M < 0 || p.K < 1) return api_fail(TKB_ERR_INVALID_ARG, "%s: need M >= 0 and K >= 1 (got M=%d K=%d)", what, p.M, p.K);
+    if (p.M < 0 || p.M > kMaxRows || p.K < 1) return api_fail(TKB_ERR_INVALID_ARG, "%s: need 0 <= M <= 2^30 and K >= 1 (got M=%d K=%d)", what, p.M, p.K);
     const int max_k = mode == ROWS_QUANT ? kQuantMaxK : kNormMaxK;
     if (p.K > max_k) return api_fail(TKB_ERR_INVALID_ARG, "%s: K=%d is above %d, the longest row that one CTA holds", what, p.K, max_k);
     if ((p.codes == nullptr) != (p.sc == nullptr) && p.M > 0) return api_fail(TKB_ERR_INVALID_ARG, "%s: int8 codes and their scales come together", what);
@@ -532,16 +532,20 @@ static int rows_call(const char* what, RowsParams p, int mode, int dtype, void* 
     if (reinterpret_cast<uintptr_t>(p.sc) & 3u) return api_fail(TKB_ERR_BAD_ALIGNMENT, "%s: scales must be 4-byte aligned", what);
     if (p.M == 0) return TKB_OK;
     // outputs may not touch anything else, but for r, which may be x itself
-    const int64_t row = int64_t(p.K) * 2;
-    const Span in[2] = {{"x", p.x, p.ldx * 2, row}, {"h", p.h, p.ldh * 2, row}};
-    const Span out[3] = {{"r", p.r, p.ldr * 2, row}, {"y", p.y, p.ldy * 2, row}, {"codes", p.codes, p.ldc, p.K}};
-    for (int i = 0; i < 3; i++) {
+    const int64_t row = int64_t(p.K) * 2, gates = p.gate ? (int64_t(p.M) + p.rows_per_gate - 1) / p.rows_per_gate : 1;
+    const Span in[5] = {{"x", p.x, p.M, p.ldx * 2, row}, {"h", p.h, p.M, p.ldh * 2, row}, {"gate", p.gate, gates, p.ldg * 2, row},
+                        {"the weight after the block", p.w_post, 1, row, row}, {"the weight", p.w_pre, 1, row, row}};
+    const Span out[4] = {{"r", p.r, p.M, p.ldr * 2, row}, {"y", p.y, p.M, p.ldy * 2, row}, {"codes", p.codes, p.M, p.ldc, p.K},
+                         {"scales", p.sc, 1, int64_t(p.M) * 4, int64_t(p.M) * 4}};
+    for (int i = 0; i < 4; i++) {
         for (const Span& s : in)
-            if (overlap(out[i], s, p.M) && !(i == 0 && s.ptr == p.x && out[i].ptr == p.x && out[i].pitch == s.pitch))
+            if (overlap(out[i], s) && !(i == 0 && s.ptr == p.x && out[i].ptr == p.x && out[i].pitch == s.pitch))
                 return api_fail(TKB_ERR_INVALID_ARG, "%s: output %s overlaps input %s", what, out[i].name, s.name);
         for (int k = 0; k < i; k++)
-            if (overlap(out[i], out[k], p.M)) return api_fail(TKB_ERR_INVALID_ARG, "%s: outputs %s and %s overlap", what, out[i].name, out[k].name);
+            if (overlap(out[i], out[k])) return api_fail(TKB_ERR_INVALID_ARG, "%s: outputs %s and %s overlap", what, out[i].name, out[k].name);
     }
+    // 16-byte accesses where every row of every 16-bit tensor begins on 16 bytes (codes: on 8) and holds whole groups of 8, or where the
+    // rows of all of them begin alike within 16 bytes
     // (a longest row that begins inside a group would need one group more than there are)
     const bool one = p.M == 1;
     auto whole = [&](const void* q, int64_t ld) { return !q || one || ld % 8 == 0; };
