@@ -189,37 +189,48 @@ def _bad(t, name: str, dtypes, device, shape) -> None:
     raise RuntimeError(f"{name} must have a contiguous last dimension and rows that do not overlap")
 
 
-# The checks below run before every launch and count where a call takes microseconds: each asks a tensor once for each property.
+# The checks below run before every launch and count where a call takes microseconds: each asks a tensor once for each property, and
+# what is no tensor, or has other dimensions, is told apart only once something is wrong.
+_NO_TENSOR = (AttributeError, TypeError, ValueError)
+
 
 def _first(t, name: str, dtypes):
     """Checks the matrix that fixes a call's rows, columns and device: (rows, columns, device, row pitch in elements)."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes or t.dim() != 2:
-        _bad(t, name, dtypes, None, (None, None))
-    n, k = t.shape
-    pitch, step = t.stride()
-    if n <= 1:                              # no pitch that anything reads
-        pitch = k
-    if pitch < k or (step != 1 and k > 1):
-        _bad(t, name, dtypes, None, (n, k))
-    return n, k, t.get_device(), pitch
+    try:
+        n, k = t.shape
+        pitch, step = t.stride()
+        device = t.get_device()
+        if n <= 1:                          # no pitch that anything reads
+            pitch = k
+        if device >= 0 and t.dtype in dtypes and pitch >= k and (step == 1 or k <= 1):
+            return n, k, device, pitch
+    except _NO_TENSOR:
+        pass
+    _bad(t, name, dtypes, None, (None, None))
 
 
 def _mat(t, name: str, dtypes, device: int, n: int, k: int) -> int:
     """Checks a row-strided [n, k] matrix and returns its row pitch in elements."""
-    if isinstance(t, torch.Tensor) and t.get_device() == device and t.dtype in dtypes and t.shape == (n, k):
-        pitch, step = t.stride()
-        if n <= 1:
-            pitch = k
-        if pitch >= k and (step == 1 or k <= 1):
-            return pitch
+    try:
+        if t.get_device() == device and t.dtype in dtypes and t.shape == (n, k):
+            pitch, step = t.stride()
+            if n <= 1:
+                pitch = k
+            if pitch >= k and (step == 1 or k <= 1):
+                return pitch
+    except _NO_TENSOR:
+        pass
     _bad(t, name, dtypes, device, (n, k))
 
 
 def _vec(t, name: str, dtypes, device: int, n: int) -> int:
     """Checks a contiguous vector and returns its address."""
-    if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dtype not in dtypes or t.shape != (n,) or not t.is_contiguous():
-        _bad(t, name, dtypes, device, (n,))
-    return t.data_ptr()
+    try:
+        if t.get_device() == device and t.dtype in dtypes and t.shape == (n,) and t.is_contiguous():
+            return t.data_ptr()
+    except _NO_TENSOR:
+        pass
+    _bad(t, name, dtypes, device, (n,))
 
 
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
