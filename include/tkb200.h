@@ -135,15 +135,16 @@ int tkb_mxfp8_quantize(const void* A_bf16, int64_t lda, void* codes, void* sc, i
  * channels).  For every row  amax = max(max_k |A|, 2^-100),  sc = fl32(amax / 127),  codes = rint(A * fl32(127 / amax)), the
  * product exact and rounded half to even, so |codes| <= 127.  A row that holds an infinity or a NaN gets sc = NaN and codes 0.
  *   A [M, K] of `dtype` (bf16 or fp16), row pitch lda elements (0 = K); codes [M, K] int8, row pitch ldc bytes (0 = K; what lies
- *   between K and ldc is left alone); sc [M] fp32.  Any M >= 0, 1 <= K <= 65536, any alignment; codes may not overlap A.
+ *   between K and ldc is left alone); sc [M] fp32.  0 <= M <= 2^30, 1 <= K <= 65536, any alignment; A, codes and sc may not overlap.
  * No counterpart in the reference. */
 int tkb_int8_quantize(const void* A, int64_t lda, int dtype, void* codes, int64_t ldc, float* sc, int M, int K, void* stream);
 
 /* The norm before a block:  y = x * rsqrt(mean_k x^2 + eps) * W.  It leaves as Y [M, K] of `dtype`, as codes [M, K] int8 with
  * sc [M] fp32 (quantized from the unrounded y as in tkb_int8_quantize), or as both; a NULL output is not written.
- *   X, Y [M, K], W [K], all of `dtype` (bf16 or fp16); row pitches in elements (0 = K).  Any M >= 0, 1 <= K <= 16384, any
- *   alignment (16-byte aligned rows and K % 8 == 0 are read fastest).  Sums and y are held in fp32: |x| above about 1e19
- *   overflows its square.  Outputs may not overlap X or one another.
+ *   X, Y [M, K], W [K], all of `dtype` (bf16 or fp16); row pitches in elements (0 = K).  0 <= M <= 2^30, 1 <= K <= 16384, any
+ *   alignment (16-byte aligned rows and K % 8 == 0 go fastest, next rows of all tensors that begin alike within 16 bytes).  Sums and
+ *   y are held in fp32: |x| above about 1e19 overflows its square.  Outputs may not overlap an input or one another.  Y and the
+ *   codes are the same whether one or both are asked for.
  * No counterpart in the reference. */
 int tkb_rms_norm(const void* X, int64_t ldx, const void* W, void* Y, int64_t ldy, void* codes, int64_t ldc, float* sc, int dtype, int M, int K,
                  float eps, void* stream);
@@ -154,8 +155,8 @@ int tkb_rms_norm(const void* X, int64_t ldx, const void* W, void* Y, int64_t ldy
  *   y = r * rsqrt(mean_k r^2 + eps) * W_pre      (left out if W_pre is NULL)    -> Y and / or codes, sc as in tkb_rms_norm
  *   H (the block's output), X (the residual stream), R, Y [M, K], W_post, W_pre [K] and gate of `dtype`; row i uses gate row
  *   i / rows_per_gate of pitch ldg: one gate for all (rows_per_gate >= M), one for each sequence of a batch, one for each token.
- *   y is made from the unrounded r.  R may be X itself (same pointer and pitch); otherwise outputs may not overlap H, X or one
- *   another.  Sizes, pitches and precision as in tkb_rms_norm.
+ *   y is made from the unrounded r.  R may be X itself (same pointer and pitch); otherwise outputs may not overlap an input or one
+ *   another.  residual_scale is a finite number.  Sizes, pitches and precision as in tkb_rms_norm.
  * No counterpart in the reference. */
 int tkb_block_norm(const void* H, int64_t ldh, const void* X, int64_t ldx, void* R, int64_t ldr, const void* W_post, const void* gate, int64_t ldg,
                    int rows_per_gate, float residual_scale, const void* W_pre, void* Y, int64_t ldy, void* codes, int64_t ldc, float* sc,
@@ -224,9 +225,11 @@ int tkb_fp8_gemm_ex(const void* A, int64_t lda, const void* B, int64_t ldb, void
  *   D[m, n] = A_sc[m] * B_sc[n] * sum_k A[m, k] * B[n, k]
  *   A [M, K], B [N, K] int8, row pitches lda / ldb bytes (0 = K; multiples of 16, 16-byte aligned bases; lda is free when M == 1);
  *   A_sc [M], B_sc [N] fp32; D [M, N] of `dtype` (bf16, fp16 or fp32), row pitch ldd elements (0 = N), any alignment.
- *   Any M >= 0, N >= 1, 1 <= K <= 131071 (the sum is exact in int32), odd ones too.  The sum is converted to fp32, multiplied by
- *   A_sc[m], then by B_sc[n], and rounded to `dtype`; results do not depend on the run, the tile or the split of K.
- * The _ex form takes TKB_GEMM_* tiles (the skinny and the 512-row ones belong to other formats).  No counterpart in the reference. */
+ *   Any M >= 0, N >= 1, 1 <= K <= 131071 (the sum is exact in int32), odd ones too; M, N <= 2^30.  The sum is converted to fp32,
+ *   multiplied by A_sc[m], then by B_sc[n], and rounded to `dtype`: results depend neither on the run nor on the kernel or tile that
+ *   the sizes choose.  D may not overlap the operands.  No scratch: calls on any streams and captured graphs are independent.
+ * Up to 128 tokens stream the weights once (one of two kernels, by N); more go through the GEMM tiles.  The _ex form takes
+ * TKB_GEMM_PAIR_N256 .. TKB_GEMM_SINGLE_N128 for any M.  No counterpart in the reference. */
 int tkb_int8_gemm(const void* A, int64_t lda, const float* A_sc, const void* B, int64_t ldb, const float* B_sc, void* D, int64_t ldd, int dtype,
                   int M, int N, int K, void* stream);
 int tkb_int8_gemm_ex(const void* A, int64_t lda, const float* A_sc, const void* B, int64_t ldb, const float* B_sc, void* D, int64_t ldd, int dtype,
