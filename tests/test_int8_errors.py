@@ -52,6 +52,13 @@ def test_int8_gemm(lib):
     assert f(None, 0, None, B, 0, SB, None, 0, BF16, 0, 8, 64, None) == 0      # no rows
 
 
+def test_int8_gemm_output_over_an_operand(lib):
+    f = lib.tkb_int8_gemm
+    A, SA, B, SB, D = FAR[:5]
+    for D in (A, A + 8 * 64 - 2, SA + 28, SA - 126, B + 64, SB):               # 8 x 8 bf16: 128 bytes
+        assert f(A, 0, SA, B, 0, SB, D, 0, BF16, 8, 8, 64, None) == INVALID and "overlaps" in _msg(lib)
+
+
 def test_rms_norm(lib):
     f = lib.tkb_rms_norm
     X, W, Y, Q, S = FAR[:5]

@@ -346,6 +346,10 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
     const int out_bytes = dtype == TKB_DTYPE_FP32 ? 4 : 2;
     if ((reinterpret_cast<uintptr_t>(A_sc) | reinterpret_cast<uintptr_t>(B_sc)) & 3u || reinterpret_cast<uintptr_t>(D) & uintptr_t(out_bytes - 1))
         return api_fail(TKB_ERR_BAD_ALIGNMENT, "int8_gemm: scales and D must be aligned to their element type");
+    const Span out = {"D", D, M, ldd * out_bytes, int64_t(N) * out_bytes};
+    const Span in[4] = {{"A", A, M, lda, K}, {"A_sc", A_sc, 1, int64_t(M) * 4, int64_t(M) * 4}, {"B", B, N, ldb, K}, {"B_sc", B_sc, 1, int64_t(N) * 4, int64_t(N) * 4}};
+    for (const Span& s : in)
+        if (overlap(out, s)) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: D overlaps %s", s.name);
     DeviceCtx* c;
     if (int e = get_ctx(&c)) return e;
     if (M <= kInt8SkinnyMaxM && config == TKB_GEMM_DEFAULT) {

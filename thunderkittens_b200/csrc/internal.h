@@ -103,6 +103,10 @@ struct DecodeArgs {
 cudaError_t launch_decode(const DecodeArgs& a);
 int decode_padded_rows(int M);
 
+// norm.cu
+struct Span { const char* name; const void* ptr; int64_t rows, pitch, width; };     // a row-strided buffer; pitch, width in bytes
+bool overlap(const Span& a, const Span& b);
+
 // int8_skinny.cu
 constexpr int kInt8SkinnyMaxM = 128;
 struct SkinnyArgs {

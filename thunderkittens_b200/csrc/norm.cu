@@ -494,10 +494,8 @@ static cudaError_t launch_rows_t(const RowsParams& p, int kind, int sm_count, cu
 }
 
 // ---- argument checks ------------------------------------------------------------------------
-struct Span { const char* name; const void* ptr; int64_t rows, pitch, width; };     // pitch, width in bytes
-
 // Whether two row-strided buffers share a byte.  Column slices of one buffer (equal pitches) interleave without touching.
-static bool overlap(const Span& a, const Span& b) {
+bool overlap(const Span& a, const Span& b) {
     if (!a.ptr || !b.ptr) return false;
     const uintptr_t pa = reinterpret_cast<uintptr_t>(a.ptr), pb = reinterpret_cast<uintptr_t>(b.ptr);
     if (pa + uintptr_t((a.rows - 1) * a.pitch + a.width) <= pb || pb + uintptr_t((b.rows - 1) * b.pitch + b.width) <= pa) return false;
