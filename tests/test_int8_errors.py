@@ -116,3 +116,23 @@ def test_ops_refuse_tensors_off_the_gpu():
         ops.rms_norm(x, x[0], x.clone())
     with pytest.raises(RuntimeError, match="must be a torch.Tensor"):
         ops.block_norm(None, x, x)
+
+
+def test_ops_refuse_sizes_past_c_ints():
+    """2^32 + 4 rows would arrive as 4."""
+    import torch
+    from thunderkittens_b200 import ops
+
+    class Sized(torch.Tensor):               # a size on a CUDA device, and no memory
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise AssertionError(f"{func} on a tensor without memory")
+
+    def sized(shape, dtype):
+        return torch.Tensor._make_wrapper_subclass(Sized, shape, dtype=dtype, device="cuda:0")
+
+    for M, K in ((2 ** 32 + 4, 1), (4, 2 ** 32 + 16)):
+        with pytest.raises(RuntimeError, match="sizes up to"):
+            ops.int8_quantize(sized((M, K), torch.bfloat16), sized((M, K), torch.int8), sized((M,), torch.float32))
+        with pytest.raises(RuntimeError, match="sizes up to"):
+            ops.rms_norm(sized((M, K), torch.float16), sized((K,), torch.float16), sized((M, K), torch.float16))

@@ -184,6 +184,8 @@ def _bad(t, name: str, dtypes, device, shape) -> None:
         raise RuntimeError(f"{name} has dtype {t.dtype}, expected one of {tuple(dtypes)}")
     if device is not None and t.get_device() != device:
         raise RuntimeError(f"{name} is on device {t.get_device()}, the first operand on device {device}")
+    if max(t.shape, default=0) > _MAX_SIZE:
+        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, of which the library takes sizes up to {_MAX_SIZE}")
     if t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
         raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple('any' if s is None else s for s in shape)}")
     raise RuntimeError(f"{name} must have a contiguous last dimension and rows that do not overlap")
@@ -192,6 +194,7 @@ def _bad(t, name: str, dtypes, device, shape) -> None:
 # The checks below run before every launch and count where a call takes microseconds: each asks a tensor once for each property, and
 # what is no tensor, or has other dimensions, is told apart only once something is wrong.
 _NO_TENSOR = (AttributeError, TypeError, ValueError)
+_MAX_SIZE = 2 ** 31 - 1                     # sizes are passed as C ints, which would keep the low 32 bits of a larger one
 
 
 def _first(t, name: str, dtypes):
@@ -202,7 +205,7 @@ def _first(t, name: str, dtypes):
         device = t.get_device()
         if n <= 1:                          # no pitch that anything reads
             pitch = k
-        if device >= 0 and t.dtype in dtypes and pitch >= k and (step == 1 or k <= 1):
+        if device >= 0 and t.dtype in dtypes and n <= _MAX_SIZE and k <= pitch and k <= _MAX_SIZE and (step == 1 or k <= 1):
             return n, k, device, pitch
     except _NO_TENSOR:
         pass
