@@ -1,4 +1,5 @@
-"""Builds thunderkittens_b200/libtkb200.so from csrc/*.cu with nvcc for sm_100a (in-tree).
+"""Builds thunderkittens_b200/libtkb200.so from csrc/*.cu with nvcc for sm_100a, and on top of it the Python module
+thunderkittens_b200/_torch_ops.so from csrc/torch_ops.cpp with the host compiler (in-tree).
 
     python -m thunderkittens_b200.build [--force] [--verbose]
 
@@ -9,12 +10,14 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_obj")
 LIB = os.path.join(HERE, "libtkb200.so")
+TORCH_OPS = os.path.join(HERE, "_torch_ops.so")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
@@ -30,7 +33,7 @@ def sources() -> list[str]:
 
 def _deps() -> list[str]:
     inc = os.path.join(os.path.dirname(HERE), "include")
-    return [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(inc, f) for f in os.listdir(inc)] + [__file__]
+    return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".cpp")] + [os.path.join(inc, f) for f in os.listdir(inc)] + [__file__]
 
 
 def _compile(src: str, force: bool, verbose: bool) -> str:
@@ -60,7 +63,26 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    _build_torch_ops(force)
     return LIB
+
+
+def _build_torch_ops(force: bool) -> None:
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    deps = [src, os.path.join(os.path.dirname(HERE), "include", "tkb200.h"), __file__]
+    if not force and os.path.exists(TORCH_OPS) and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_OPS) for d in deps):
+        return
+    import torch
+    torch_dir = os.path.dirname(torch.__file__)
+    include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(CUDA_HOME, "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(a for d in include for a in ("-isystem", d)), src, "-o", TORCH_OPS, "-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
+           "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed on torch_ops.cpp")
 
 
 if __name__ == "__main__":

@@ -168,87 +168,17 @@ def nvfp4_gemm_quant(A, A_sc, A_sg, B, B_sc, B_sg, out_amax, D_codes, D_sc, D_sg
 # Unlike the entries above these take row-strided tensors (last dimension contiguous), run on the device of their
 # tensors, whichever is current, on that device's current stream, and accept no rows at all.
 
-_HALF = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_FP16}
-_OUT = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_FP16, torch.float32: L.DTYPE_FP32}
-_INT8 = (torch.int8,)
-_FP32 = (torch.float32,)
+_torch_ops = None
 
 
-def _bad(t, name: str, dtypes, device, shape) -> None:
-    """Raises the error that _mat or _vec found."""
-    if not isinstance(t, torch.Tensor):
-        raise RuntimeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor")
-    if t.dtype not in dtypes:
-        raise RuntimeError(f"{name} has dtype {t.dtype}, expected one of {tuple(dtypes)}")
-    if device is not None and t.get_device() != device:
-        raise RuntimeError(f"{name} is on device {t.get_device()}, the first operand on device {device}")
-    if max(t.shape, default=0) > _MAX_SIZE:
-        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, of which the library takes sizes up to {_MAX_SIZE}")
-    if t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
-        raise RuntimeError(f"{name} has shape {tuple(t.shape)}, expected {tuple('any' if s is None else s for s in shape)}")
-    raise RuntimeError(f"{name} must have a contiguous last dimension and rows that do not overlap")
-
-
-# The checks below run before every launch and count where a call takes microseconds: each asks a tensor once for each property, and
-# what is no tensor, or has other dimensions, is told apart only once something is wrong.
-_NO_TENSOR = (AttributeError, TypeError, ValueError)
-_MAX_SIZE = 2 ** 31 - 1                     # sizes are passed as C ints, which would keep the low 32 bits of a larger one
-
-
-def _first(t, name: str, dtypes):
-    """Checks the matrix that fixes a call's rows, columns and device: (rows, columns, device, row pitch in elements)."""
-    try:
-        n, k = t.shape
-        pitch, step = t.stride()
-        device = t.get_device()
-        if n <= 1:                          # no pitch that anything reads
-            pitch = k
-        if device >= 0 and t.dtype in dtypes and n <= _MAX_SIZE and k <= pitch and k <= _MAX_SIZE and (step == 1 or k <= 1):
-            return n, k, device, pitch
-    except _NO_TENSOR:
-        pass
-    _bad(t, name, dtypes, None, (None, None))
-
-
-def _mat(t, name: str, dtypes, device: int, n: int, k: int) -> int:
-    """Checks a row-strided [n, k] matrix and returns its row pitch in elements."""
-    try:
-        if t.get_device() == device and t.dtype in dtypes and t.shape == (n, k):
-            pitch, step = t.stride()
-            if n <= 1:
-                pitch = k
-            if pitch >= k and (step == 1 or k <= 1):
-                return pitch
-    except _NO_TENSOR:
-        pass
-    _bad(t, name, dtypes, device, (n, k))
-
-
-def _vec(t, name: str, dtypes, device: int, n: int) -> int:
-    """Checks a contiguous vector and returns its address."""
-    try:
-        if t.get_device() == device and t.dtype in dtypes and t.shape == (n,) and t.is_contiguous():
-            return t.data_ptr()
-    except _NO_TENSOR:
-        pass
-    _bad(t, name, dtypes, device, (n,))
-
-
-_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-
-
-def _call(device: int, entry, *args) -> None:
-    """Calls an entry on the current stream of `device` (its handle alone: torch.cuda.current_stream() builds a Stream object
-    around it, 3 us; a tensor of the call is on the GPU, so CUDA is initialised)."""
-    if _current_device() == device:
-        code = entry(*args, _current_stream(device))
-    else:
-        with torch.cuda.device(device):
-            code = entry(*args, _current_stream(device))
-    if code:
-        L.check(code)
+def _native():
+    """The module that checks these calls' tensors and launches them; raises if it has not been built."""
+    global _torch_ops
+    if _torch_ops is None:
+        L.lib()
+        from . import _torch_ops as module
+        _torch_ops = module
+    return _torch_ops
 
 
 def int8_quantize(A, A_int8, A_sc) -> None:
@@ -257,48 +187,23 @@ def int8_quantize(A, A_int8, A_sc) -> None:
     A_sc = max(amax, 2**-100) / 127 and A_int8 = rint(A * (127 / amax)), the inverse step in fp32 and the product exact; a row that
     holds an infinity or a NaN gets step NaN and codes 0.  K <= 65536.  As an operand of int8_gemm the rows of A_int8 must begin
     16 bytes apart: for other K allocate (M, K rounded up to 16) and pass the [:, :K] slice."""
-    M, K, dev, lda = _first(A, "A", _HALF)
-    ldc = _mat(A_int8, "A_int8", _INT8, dev, M, K)
-    _call(dev, L.lib().tkb_int8_quantize, A.data_ptr(), lda, _HALF[A.dtype], A_int8.data_ptr(), ldc, _vec(A_sc, "A_sc", _FP32, dev, M), M, K)
+    if code := _native().int8_quantize(A, A_int8, A_sc):
+        L.check(code)
 
 
 def int8_gemm(A, A_sc, B, B_sc, D, config: str | None = None) -> None:
     """D (M,N) = A_sc[:, None] * B_sc * (A @ B.T); A (M,K), B (N,K) int8, A_sc (M,), B_sc (N,) fp32, D bf16, fp16 or fp32.
 
     The sums are exact (K <= 131071).  Rows of A and B begin 16 bytes apart; D may have any row pitch."""
-    M, K, dev, lda = _first(A, "A", _INT8)
-    N, KB, devB, ldb = _first(B, "B", _INT8)
-    if KB != K or devB != dev:
-        _bad(B, "B", _INT8, dev, (None, K))
-    ldd = _mat(D, "D", _OUT, dev, M, N)
-    _call(dev, L.lib().tkb_int8_gemm_ex, A.data_ptr(), lda, _vec(A_sc, "A_sc", _FP32, dev, M), B.data_ptr(), ldb, _vec(B_sc, "B_sc", _FP32, dev, N),
-          D.data_ptr(), ldd, _OUT[D.dtype], M, N, K, _CONFIG[config])
-
-
-def _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc):
-    """Arguments of the optional outputs of a norm: Y, its pitch, the codes, their pitch, their steps."""
-    y = ldy = q = ldq = sc = 0
-    if Y is not None:
-        ldy = _mat(Y, "Y", (t,), dev, M, K)
-        y = Y.data_ptr()
-    if (Y_int8 is None) != (Y_sc is None):
-        raise RuntimeError("Y_int8 and Y_sc come together")
-    if Y_int8 is not None:
-        ldq = _mat(Y_int8, "Y_int8", _INT8, dev, M, K)
-        q, sc = Y_int8.data_ptr(), _vec(Y_sc, "Y_sc", _FP32, dev, M)
-    return y, ldy, q, ldq, sc
+    if code := _native().int8_gemm(A, A_sc, B, B_sc, D, _CONFIG[config]):
+        L.check(code)
 
 
 def rms_norm(X, W, Y=None, Y_int8=None, Y_sc=None, eps: float = 1e-6) -> None:
     """y = X * rsqrt(mean(X**2) + eps) * W over the rows of X (M,K) bf16 or fp16, K <= 16384, into Y (M,K) of X's dtype and / or,
     quantized as by int8_quantize, into Y_int8 (M,K) and Y_sc (M,)."""
-    M, K, dev, ldx = _first(X, "X", _HALF)
-    t = X.dtype
-    w = _vec(W, "W", (t,), dev, K)
-    if Y is None and Y_int8 is None:
-        raise RuntimeError("rms_norm needs Y or Y_int8 and Y_sc")
-    y, ldy, q, ldq, sc = _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc)
-    _call(dev, L.lib().tkb_rms_norm, X.data_ptr(), ldx, w, y, ldy, q, ldq, sc, _HALF[t], M, K, eps)
+    if code := _native().rms_norm(X, W, Y, Y_int8, Y_sc, eps):
+        L.check(code)
 
 
 def block_norm(H, X, X_out, W_post=None, gate=None, residual_scale: float = 1.0, W_pre=None, Y=None, Y_int8=None, Y_sc=None,
@@ -310,28 +215,5 @@ def block_norm(H, X, X_out, W_post=None, gate=None, residual_scale: float = 1.0,
 
     gate is (K,), or (G,K) with M a multiple of G: row i uses gate row i // (M // G), that is one gate for each sequence of a
     batch, or with G = M one for each token.  X_out may be X."""
-    M, K, dev, ldh = _first(H, "H", _HALF)
-    t = H.dtype
-    ldx = _mat(X, "X", (t,), dev, M, K)
-    ldr = _mat(X_out, "X_out", (t,), dev, M, K)
-    w_post = 0 if W_post is None else _vec(W_post, "W_post", (t,), dev, K)
-    w_pre = 0 if W_pre is None else _vec(W_pre, "W_pre", (t,), dev, K)
-    g = ldg = 0
-    per = 1
-    if gate is not None:
-        if isinstance(gate, torch.Tensor) and gate.dim() == 1:
-            g, ldg, per = _vec(gate, "gate", (t,), dev, K), K, max(M, 1)
-        else:
-            G, KG, devG, ldg = _first(gate, "gate", (t,))
-            if KG != K or devG != dev:
-                _bad(gate, "gate", (t,), dev, (None, K))
-            if (M % G if G else M) or (M and M < G):
-                raise RuntimeError(f"gate has {G} rows, of which {M} rows of H are no multiple")
-            g, per = gate.data_ptr(), max(M // G, 1) if G else 1
-    if W_pre is None and (Y is not None or Y_int8 is not None):
-        raise RuntimeError("Y and Y_int8 need W_pre")
-    if W_pre is not None and Y is None and Y_int8 is None:
-        raise RuntimeError("W_pre needs Y or Y_int8 and Y_sc")
-    y, ldy, q, ldq, sc = _norm_outputs(dev, M, K, t, Y, Y_int8, Y_sc)
-    _call(dev, L.lib().tkb_block_norm, H.data_ptr(), ldh, X.data_ptr(), ldx, X_out.data_ptr(), ldr, w_post, g, ldg, per, residual_scale,
-          w_pre, y, ldy, q, ldq, sc, _HALF[t], M, K, eps)
+    if code := _native().block_norm(H, X, X_out, W_post, gate, residual_scale, W_pre, Y, Y_int8, Y_sc, eps):
+        L.check(code)
