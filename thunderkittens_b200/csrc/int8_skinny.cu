@@ -4,12 +4,13 @@
 // anything but D in global memory, so that calls on any number of streams and captured graphs do not meet:
 //
 // Long streams: operands are swapped as in the NVFP4 decode kernel (decode.cu): weight rows are the M side of a tcgen05.mma (128
-// lanes), the tokens, padded to 16 / 32 / 64 / 128, its N side.  What matters is that every SM streams the same number of bytes
+// lanes), the tokens its N side.  What matters is that every SM streams the same number of bytes
 // without a gap:
+//   * tokens are padded to the next multiple of 16 only;
 //   * slabs have R <= 128 weight rows, R chosen so that they divide evenly over the SMs (a TMA box may have any number of rows;
 //     the lanes past R multiply whatever is in shared memory and are not read).  N = 28672: two slabs of 97 rows for each SM;
 //   * a CTA walks over its slabs; two accumulators in tensor memory, so that the epilogue of a slab overlaps the next one's loads;
-//   * warp 0 = TMA producer, warp 1 = MMA issuer + tensor-memory owner, warps 2..5 = epilogue.
+//   * warp 0 = TMA producer, warp 1 = MMA issuer + tensor-memory owner, warps 2..9 = epilogue.
 //
 // Short streams: an SM's share of the weights is a few dozen KB, and a single pass through TMA, barriers and tensor memory costs
 // more than the bytes.  A CTA takes 16 rows; its warps take 128-byte pieces of K in turn, straight from global memory into the
@@ -23,15 +24,7 @@ namespace tkb {
 
 constexpr int kSkinnyStages = 16;
 constexpr int kSkinnySmem = 208 * 1024;
-
-template <int NB>
-struct SkinnyCfg {
-    static constexpr int X_BYTES = NB * 128;
-    static constexpr int ACC_COLS = NB < 32 ? 32 : NB;   // of one accumulator
-    static constexpr int TMEM_COLS = 2 * ACC_COLS;
-    static constexpr int THREADS = 6 * 32;
-    static constexpr int CHUNK = NB < 32 ? 16 : 32;      // accumulator columns read per tcgen05.ld
-};
+constexpr int kSkinnyThreads = 10 * 32;
 
 struct SkinnyParams {
     const float* a_sc; const float* b_sc;
@@ -39,34 +32,35 @@ struct SkinnyParams {
     const uint8_t* B; int64_t ldb;
     int M, N, K, out_dtype;
     int rows, slabs;                        // weight rows of a slab, slabs
-    int stages, w_bytes;                    // operand ring: stages, bytes from one stage's weights to the next's
+    int nb, acc_cols;                       // tokens padded to the MMA's N; tensor-memory columns of an accumulator
+    int group, stages, w_bytes;             // operand ring: 128-byte blocks of K of a stage, stages, bytes from one block's weights to the next's
     int prefetch;                           // 128-byte pieces of its weights that a CTA asks L2 for early
     int* status;
     long long wait_limit;
 };
 
-__device__ __forceinline__ void tmem_ld_32x16_i(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
+// The same wait as mbar_wait, whose slow path stays out of the loops of one thread: they would run over it (see below)
+__device__ __noinline__ bool skinny_wait_slow(int* abort_flag, int* status, long long limit, uint32_t bar, uint32_t parity) {
+    return mbar_wait(WaitCtx{abort_flag, status, limit}, bar, parity);
 }
 
-__device__ __forceinline__ void store_out(const SkinnyParams& p, int m, int n, int sum, float a_sc, float b_sc) {
-    const float v = __int2float_rn(sum) * a_sc * b_sc;
-    const int64_t at = int64_t(m) * p.ldd + n;
-    if (p.out_dtype == TKB_DTYPE_FP32) static_cast<float*>(p.D)[at] = v;
-    else if (p.out_dtype == TKB_DTYPE_FP16) static_cast<__half*>(p.D)[at] = __float2half_rn(v);
-    else static_cast<__nv_bfloat16*>(p.D)[at] = __float2bfloat16_rn(v);
+__device__ __forceinline__ float scaled(int sum, float a_sc, float b_sc) { return __int2float_rn(sum) * a_sc * b_sc; }
+__device__ __forceinline__ void put(float* d, float v) { *d = v; }
+__device__ __forceinline__ void put(__half* d, float v) { *d = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* d, float v) { *d = __float2bfloat16_rn(v); }
+// Calls f with D as a pointer to its type
+template <typename F>
+__device__ __forceinline__ void typed_out(const SkinnyParams& p, F f) {
+    if (p.out_dtype == TKB_DTYPE_FP32) f(static_cast<float*>(p.D));
+    else if (p.out_dtype == TKB_DTYPE_FP16) f(static_cast<__half*>(p.D));
+    else f(static_cast<__nv_bfloat16*>(p.D));
 }
 
-template <int NB>
-__global__ void __launch_bounds__(SkinnyCfg<NB>::THREADS)
+// GROUP blocks of K share a stage and its barriers, since what the producer's and the MMA issuer's threads spend on a turn of their loops
+// bounds slabs of few rows: M=1 N=1000 K=8192 (64 blocks) 16.1 us with 1 block, 12.6 with 2, 10.6 with 4, 10.1 with waits out of line.
+template <int GROUP>
+__global__ void __launch_bounds__(kSkinnyThreads)
 int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const SkinnyParams p) {
-    using C = SkinnyCfg<NB>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_full[kSkinnyStages];
     __shared__ __align__(8) uint64_t bar_empty[kSkinnyStages];
@@ -74,51 +68,60 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     __shared__ __align__(8) uint64_t bar_acc_empty[2];
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_abort;
+    __shared__ float s_a_sc[128];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int nst = p.stages;
-    const uint32_t sX = (smem_u32(smem_raw) + 1023u) & ~1023u;      // tokens first: an MMA reads 128 rows from a stage's weights on
-    const uint32_t sW = sX + nst * C::X_BYTES;
+    const uint32_t x_bytes = uint32_t(p.nb) * 128u, w_bytes = uint32_t(p.w_bytes);
+    const uint32_t sX = (smem_u32(smem_raw) + 1023u) & ~1023u;      // tokens first: an MMA reads 128 rows from a block's weights on
+    const uint32_t sW = sX + nst * GROUP * x_bytes;
     const int unit = int(blockIdx.x), units = int(gridDim.x);
     const int kblk = (p.K + 127) / 128;
+    const uint32_t tmem_cols = p.acc_cols <= 32 ? 64u : (p.acc_cols <= 64 ? 128u : 256u);       // two accumulators
 
     if (threadIdx.x == 0) {
         s_abort = 0;
         for (int s = 0; s < nst; s++) { mbar_init(smem_u32(&bar_full[s]), 1); mbar_init(smem_u32(&bar_empty[s]), 1); }
-        for (int b = 0; b < 2; b++) { mbar_init(smem_u32(&bar_acc_full[b]), 1); mbar_init(smem_u32(&bar_acc_empty[b]), 4); }
+        for (int b = 0; b < 2; b++) { mbar_init(smem_u32(&bar_acc_full[b]), 1); mbar_init(smem_u32(&bar_acc_empty[b]), 8); }
         fence_mbar_init();
         prefetch_tensormap(&tmW); prefetch_tensormap(&tmX);
     }
     if (warp == 1) {
-        tmem_alloc<1>(smem_u32(&s_tmem_base), C::TMEM_COLS);
+        tmem_alloc<1>(smem_u32(&s_tmem_base), tmem_cols);
         tmem_relinquish<1>();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = s_tmem_base;
-    WaitCtx wc{&s_abort, p.status, p.wait_limit};
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return mbar_try_wait(smem_u32(bar), parity) || skinny_wait_slow(&s_abort, p.status, p.wait_limit, smem_u32(bar), parity);
+    };
 
     if (warp == 0) {
         if (elect_one()) {
             uint32_t stage = 0, phase = 0, issued = 0;
             bool ok = true;
             asm volatile("griddepcontrol.wait;" ::: "memory");      // the tokens come from the kernel before this one
-            const uint32_t tx = uint32_t(p.rows) * 128u + C::X_BYTES;
+            const uint32_t tx = uint32_t(p.rows) * 128u + x_bytes;
             for (int slab = unit; slab < p.slabs && ok; slab += units)
-                for (int kb = 0; kb < kblk; kb++) {
-                    if (!mbar_wait(wc, smem_u32(&bar_empty[stage]), phase ^ 1)) { ok = false; break; }
+                for (int kb = 0; kb < kblk; kb += GROUP) {
+                    if (!wait(&bar_empty[stage], phase ^ 1)) { ok = false; break; }
                     const uint32_t full = smem_u32(&bar_full[stage]);
-                    mbar_arrive_expect_tx(full, tx);
-                    tma_load_2d(sW + stage * p.w_bytes, &tmW, full, kb * 128, slab * p.rows);
-                    tma_load_2d(sX + stage * C::X_BYTES, &tmX, full, kb * 128, 0);
+                    mbar_arrive_expect_tx(full, tx * uint32_t(min(GROUP, kblk - kb)));
+#pragma unroll
+                    for (int g = 0; g < GROUP; g++)
+                        if (kb + g < kblk) {
+                            tma_load_2d(sW + (stage * GROUP + g) * w_bytes, &tmW, full, (kb + g) * 128, slab * p.rows);
+                            tma_load_2d(sX + (stage * GROUP + g) * x_bytes, &tmX, full, (kb + g) * 128, 0);
+                        }
                     issued++;
                     if (++stage == uint32_t(nst)) { stage = 0; phase ^= 1; }
                 }
             // this SM's loads are all on their way: the next kernel may set itself up
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             for (int s = 0; s < nst && ok; s++) {                   // stage releases of the MMA thread may still be in flight
-                ok = mbar_wait(wc, smem_u32(&bar_empty[stage]), phase ^ 1);
+                ok = wait(&bar_empty[stage], phase ^ 1);
                 if (++stage == uint32_t(nst)) { stage = 0; phase ^= 1; }
             }
             if (!ok) drain_ring(bar_full, nst, issued, p.wait_limit);
@@ -128,18 +131,22 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         if (elect_one()) {
             uint32_t stage = 0, phase = 0, seg = 0;
             bool ok = true;
+            const uint32_t idesc = idesc_int8(128, p.nb);
             for (int slab = unit; slab < p.slabs && ok; slab += units, seg++) {
-                const uint32_t buf = seg & 1u;
-                if (!mbar_wait(wc, smem_u32(&bar_acc_empty[buf]), ((seg >> 1) & 1u) ^ 1u)) { ok = false; break; }
+                const uint32_t buf = seg & 1u, acc = tmem_base + buf * p.acc_cols;
+                if (!wait(&bar_acc_empty[buf], ((seg >> 1) & 1u) ^ 1u)) { ok = false; break; }
                 tc_fence_after();
-                for (int kb = 0; kb < kblk; kb++) {
-                    if (!mbar_wait(wc, smem_u32(&bar_full[stage]), phase)) { ok = false; break; }
+                for (int kb = 0; kb < kblk; kb += GROUP) {
+                    if (!wait(&bar_full[stage], phase)) { ok = false; break; }
                     tc_fence_after();
-                    const uint64_t a_desc = smem_desc_sw128(sW + stage * p.w_bytes);
-                    const uint64_t b_desc = smem_desc_sw128(sX + stage * C::X_BYTES);
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        mma_i8<1>(tmem_base + buf * C::ACC_COLS, a_desc + 2 * j, b_desc + 2 * j, idesc_int8(128, NB), (kb > 0 || j > 0) ? 1u : 0u);
+                    for (int g = 0; g < GROUP; g++)
+                        if (kb + g < kblk) {
+                            const uint64_t a_desc = smem_desc_sw128(sW + (stage * GROUP + g) * w_bytes);
+                            const uint64_t b_desc = smem_desc_sw128(sX + (stage * GROUP + g) * x_bytes);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) mma_i8<1>(acc, a_desc + 2 * j, b_desc + 2 * j, idesc, (kb + g > 0 || j > 0) ? 1u : 0u);
+                        }
                     tc_commit<1>(smem_u32(&bar_empty[stage]));
                     if (++stage == uint32_t(nst)) { stage = 0; phase ^= 1; }
                 }
@@ -148,37 +155,40 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         }
         __syncwarp();
     } else {
-        const int quarter = warp & 3;
+        // rows of the accumulator, and every other 32 of its columns (one warp for all of them: M=48 N=50257 K=2048 20.7 us against 19.8 us,
+        // M=128 26.2 against 23.3; a warp for every 32 columns, 16 in all, 25.0 and 25.4)
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
         const int n_local = quarter * 32 + lane;
         // The first weights may be asked for before the previous kernel is done, whoever writes them: this only moves lines into L2,
         // where a later write finds them.
-        for (int i = int(threadIdx.x) - 64; i < p.prefetch; i += 128) {
+        for (int i = int(threadIdx.x) - 64; i < p.prefetch; i += 256) {
             const int kb = i / p.rows, row = unit * p.rows + i % p.rows;
             if (kb < kblk && row < p.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.B + int64_t(row) * p.ldb + kb * 128));
         }
         asm volatile("griddepcontrol.wait;" ::: "memory");          // D may still be read, and the scales written, by the kernel before this one
+        if (int(threadIdx.x) - 64 < p.M) s_a_sc[threadIdx.x - 64] = p.a_sc[threadIdx.x - 64];
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         uint32_t seg = 0;
         for (int slab = unit; slab < p.slabs; slab += units, seg++) {
             const uint32_t buf = seg & 1u;
             const int n = slab * p.rows + n_local;
             const bool mine = n_local < p.rows && n < p.N;
             const float b_sc = mine ? p.b_sc[n] : 0.f;
-            const bool full = mbar_wait(wc, smem_u32(&bar_acc_full[buf]), (seg >> 1) & 1u);
+            const bool full = wait(&bar_acc_full[buf], (seg >> 1) & 1u);
             if (!__all_sync(0xffffffffu, full)) break;              // (lanes together: the loads below are the warp's)
             tc_fence_after();
+            for (int c0 = 32 * half; c0 < p.M; c0 += 64) {                  // (an accumulator has a multiple of 32 columns)
+                uint32_t r[32];
+                __syncwarp();
+                tmem_ld_32x32(tmem_base + (uint32_t(quarter * 32) << 16) + buf * p.acc_cols + c0, r);
+                tmem_ld_wait();
+                if (mine)
+                    typed_out(p, [&](auto* D) {
+                        auto* d = D + int64_t(c0) * p.ldd + n;
 #pragma unroll
-            for (int c0 = 0; c0 < NB; c0 += C::CHUNK) {
-                if (c0 < p.M) {
-                    uint32_t r[C::CHUNK];
-                    const uint32_t at = tmem_base + (uint32_t(quarter * 32) << 16) + buf * C::ACC_COLS + c0;
-                    if constexpr (C::CHUNK == 32) tmem_ld_32x32(at, r); else tmem_ld_32x16_i(at, r);
-                    tmem_ld_wait();
-                    if (mine) {
-#pragma unroll
-                        for (int i = 0; i < C::CHUNK; i++)
-                            if (c0 + i < p.M) store_out(p, c0 + i, n, int(r[i]), p.a_sc[c0 + i], b_sc);
-                    }
-                }
+                        for (int i = 0; i < 32; i++)
+                            if (c0 + i < p.M) put(d + i * p.ldd, scaled(int(r[i]), s_a_sc[c0 + i], b_sc));
+                    });
             }
             tc_fence_before();
             __syncwarp();
@@ -188,7 +198,7 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc<1>(tmem_base, C::TMEM_COLS);
+        tmem_dealloc<1>(tmem_base, tmem_cols);
     }
 }
 
@@ -279,7 +289,8 @@ __global__ void __launch_bounds__(kShortWarps * 32) int8_short_kernel(const Shor
         int sum = 0;
 #pragma unroll
         for (int w = 0; w < kShortWarps; w++) sum += red[w * TOKENS * kShortRows + e];
-        store_out(p, m, n, sum, p.a_sc[m], p.b_sc[n]);
+        const float v = scaled(sum, p.a_sc[m], p.b_sc[n]);
+        typed_out(p, [&](auto* D) { put(D + int64_t(m) * p.ldd + n, v); });
     }
 }
 
@@ -302,25 +313,32 @@ static cudaError_t launch_dependent(const void* kern, dim3 grid, int threads, in
     return cudaLaunchKernelExC(&cfg, kern, args);
 }
 
+int int8_skinny_padded_rows(int M) { return (M + 15) / 16 * 16; }
+
 // Slabs: every SM's share of N, in as few pieces of at most 128 rows as it takes.
-static void skinny_plan(int N, int sm_count, int nb, SkinnyParams& p) {
+static void skinny_plan(int M, int N, int sm_count, SkinnyParams& p) {
     const int per_sm = ((N + 127) / 128 + sm_count - 1) / sm_count;
+    p.nb = int8_skinny_padded_rows(M);
+    p.acc_cols = (p.nb + 31) / 32 * 32;
     p.rows = (N + sm_count * per_sm - 1) / (sm_count * per_sm);
     p.slabs = (N + p.rows - 1) / p.rows;
     p.w_bytes = (p.rows * 128 + 1023) / 1024 * 1024;
-    p.stages = (kSkinnySmem - 1024 - (128 * 128 - p.w_bytes)) / (p.w_bytes + nb * 128);       // the last stage's MMAs read 128 rows
-    if (p.stages > kSkinnyStages) p.stages = kSkinnyStages;
+    // at least four stages of four blocks, or five of two: M=48 N=K=4096 (16 blocks fit) 11.7 us with 1 a stage, 10.7 with 2, 10.0 with 4;
+    // M=48 N=28672 K=8192 (9 fit) 40.1, 40.6, 42.6
+    const int blocks = (kSkinnySmem - 1024 - (128 * 128 - p.w_bytes)) / (p.w_bytes + p.nb * 128);       // the last block's MMAs read 128 rows
+    p.group = blocks >= 16 ? 4 : (blocks >= 10 ? 2 : 1);
+    p.stages = blocks / p.group < kSkinnyStages ? blocks / p.group : kSkinnyStages;
     // 256 KB, where a CTA has over 1 MB: M=16 N=28672 K=8192 38.7 us against 40.4 us; M=1 N=K=8192 16.9 us against 15.3 us
     p.prefetch = int64_t(p.rows) * per_sm * p.K > (1 << 20) ? 256 * 1024 / 128 : 0;
 }
 
-template <int NB>
+template <int GROUP>
 static cudaError_t launch_skinny_t(const SkinnyArgs& a, SkinnyParams p) {
     static std::atomic<bool> attr_set[64] = {};
     CUtensorMap tmW = a.tmW, tmX = a.tmX;
     void* args[3] = {&tmW, &tmX, &p};
-    return launch_dependent(reinterpret_cast<const void*>(int8_skinny_kernel<NB>), dim3(unsigned(p.slabs < a.sm_count ? p.slabs : a.sm_count)), SkinnyCfg<NB>::THREADS,
-                            kSkinnySmem, a.stream, args, kSkinnySmem, attr_set);
+    return launch_dependent(reinterpret_cast<const void*>(int8_skinny_kernel<GROUP>), dim3(unsigned(p.slabs < a.sm_count ? p.slabs : a.sm_count)), kSkinnyThreads, kSkinnySmem,
+                            a.stream, args, kSkinnySmem, attr_set);
 }
 
 template <int TT, bool TAIL>
@@ -339,16 +357,15 @@ static cudaError_t launch_short(const SkinnyArgs& a, const SkinnyParams& p) {
     return launch_short_t<4, TAIL>(a, p);
 }
 
-int int8_skinny_padded_rows(int M) { return M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)); }
 int int8_skinny_slab_rows(int M, int N, int sm_count) {
     SkinnyParams p;
-    skinny_plan(N, sm_count, int8_skinny_padded_rows(M), p);
+    skinny_plan(M, N, sm_count, p);
     return p.rows;
 }
-// Long streams pay about 0.2 us for each 128-byte block of K, however few weight rows an SM has; short ones read the tokens again for
-// every 16 rows.  Measured, long / short in us: M=1 N=2048 K=7168 12.7 / 5.7, M=32 14.6 / 9.5, M=64 17.6 / 18.8; M=8 N=K=4096 8.9 / 5.9,
-// M=32 10.5 / 11.2; M=4 N=7168 K=2048 6.3 / 7.6; M=16 N=K=8192 16.2 / 19.6.
-bool int8_skinny_short(int M, int N, int sm_count) { return M <= 32 && N <= (M <= 16 ? 32 : 16) * sm_count; }
+// Long streams pay about 0.1 us for each 128-byte block of K, however few weight rows an SM has; short ones read the tokens again for
+// every 16 rows.  Measured, long / short in us: M=1 N=2048 K=7168 9.4 / 5.7, M=32 10.1 / 9.3; M=8 N=K=4096 7.3 / 5.8, M=16 7.4 / 7.5;
+// M=4 N=7168 K=2048 6.1 / 7.6; M=16 N=K=8192 14.0 / 19.6.
+bool int8_skinny_short(int M, int N, int sm_count) { return M <= 32 && N <= (M <= 8 ? 32 : 16) * sm_count; }
 
 cudaError_t launch_int8_skinny(const SkinnyArgs& a) {
     SkinnyParams p = {};
@@ -357,13 +374,11 @@ cudaError_t launch_int8_skinny(const SkinnyArgs& a) {
     if (int8_skinny_short(a.M, a.N, a.sm_count)) {
         return a.K % 16 ? launch_short<true>(a, p) : launch_short<false>(a, p);
     }
-    const int nb = int8_skinny_padded_rows(a.M);
-    skinny_plan(a.N, a.sm_count, nb, p);
-    switch (nb) {
-        case 16: return launch_skinny_t<16>(a, p);
-        case 32: return launch_skinny_t<32>(a, p);
-        case 64: return launch_skinny_t<64>(a, p);
-        default: return launch_skinny_t<128>(a, p);
+    skinny_plan(a.M, a.N, a.sm_count, p);
+    switch (p.group) {
+        case 4: return launch_skinny_t<4>(a, p);
+        case 2: return launch_skinny_t<2>(a, p);
+        default: return launch_skinny_t<1>(a, p);
     }
 }
 
