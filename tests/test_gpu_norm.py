@@ -116,6 +116,22 @@ def test_block_norm_gate_for_each_sequence(cuda, lib, K, dtype):
     _check_block(x, h, w1, w2, gate, 1.0, R, Y, None, None)
 
 
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+@pytest.mark.parametrize("M,G,K", [(900, 4, 512), (900, 2, 1001), (1500, 10, 1000), (1501, 19, 777), (444, 3, 5001), (600, 2, 7168), (300, 2, 12001), (3001, 1, 303)])
+def test_block_norm_gates_of_long_sequences(cuda, lib, M, G, K, dtype):
+    """Many rows with a gate for each of a few sequences, where a CTA's rows end one sequence and begin the next."""
+    x, h, w1, w2 = _inputs(M, K, dtype, cuda, 8)
+    gate = torch.randn(G, 2 * K + 1, device=cuda).to(dtype)[:, 1:K + 1]
+    per_row = gate.repeat_interleave(M // G, 0)
+    R, Y = (torch.full((M, K), float("nan"), dtype=dtype, device=cuda) for _ in range(2))
+    q, sc = padded(M, K, torch.int8, cuda)[0], torch.empty(M, device=cuda)
+    _ops().block_norm(h, x, R, w1, gate, 0.5, w2, Y, eps=EPS)
+    _check_block(x, h, w1, w2, per_row, 0.5, R, Y, None, None)
+    X = x.clone()                                    # in place, without the first norm, quantized
+    _ops().block_norm(h, X, X, None, gate, 1.0, w2, None, q, sc, eps=EPS)
+    _check_block(x, h, None, w2, per_row, 1.0, X, None, q, sc)
+
+
 def test_strides_offsets_and_neighbours(cuda, lib):
     """Column slices of one buffer as inputs and outputs; nothing outside them is written."""
     M, K = 37, 504

@@ -31,8 +31,10 @@ enum RowsMode : int { ROWS_QUANT = 0, ROWS_NORM = 1, ROWS_BLOCK = 2 };
 //   ROWS_SINGLE   single elements, where the tensors begin differently
 enum RowsKind : int { ROWS_WHOLE = 0, ROWS_SHIFTED = 1, ROWS_SINGLE = 2 };
 // How rows share a CTA: one row each (everything that depends on the row is uniform over the CTA); a row for each warp (no barriers);
-// several groups of warps with a row each, which also share weights in shared memory
-enum RowsLayout : int { ROWS_ONE = 0, ROWS_WARPS = 1, ROWS_STAGED = 2 };
+// several groups of warps with a row each, which also share weights in shared memory; the same with rows dealt out in one piece for each
+// CTA, which meets up to two gates, each in shared memory with the weights
+enum RowsLayout : int { ROWS_ONE = 0, ROWS_WARPS = 1, ROWS_STAGED = 2, ROWS_GATES = 3 };
+constexpr int kRowsSmem = 220 * 1024;          // dynamic shared memory that a CTA may have
 constexpr int kNormMaxK = 16384, kQuantMaxK = 65536, kMaxRows = 1 << 30;
 
 struct RowsParams {
@@ -42,6 +44,7 @@ struct RowsParams {
     float* sc;
     int64_t ldx, ldh, ldg, ldr, ldy, ldc;      // elements
     int M, K, rows_per_gate;
+    int chunk;                                 // ROWS_GATES: rows of a CTA
     float residual_scale, eps;
 };
 
@@ -193,7 +196,7 @@ __device__ __forceinline__ void row_reduce(float& s, float& m, float2* part) {
     if (LAYOUT == ROWS_WARPS || nw == 1) return;
     if (lane == 0) part[threadIdx.x >> 5] = make_float2(s, m);
     // (a barrier chosen at run time takes all 16 of the CTA, so that no more than 4 CTAs fit an SM: only where rows share a CTA)
-    if (LAYOUT == ROWS_STAGED) asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.y), "r"(blockDim.x) : "memory");
+    if (LAYOUT >= ROWS_STAGED) asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.y), "r"(blockDim.x) : "memory");
     else __syncthreads();
     const float2 q = lane < nw ? part[lane] : make_float2(0.f, 0.f);
     if (SUM) s = warp_sum(q.x);
@@ -262,7 +265,7 @@ constexpr int rows_arrays(int mode) { return mode == ROWS_BLOCK ? 2 : 1; }      
 template <typename T, int MODE, int V, int KIND, int THREADS, int LAYOUT>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
     using S = Slots<V, KIND>;
-    constexpr bool STAGED = LAYOUT == ROWS_STAGED;
+    constexpr bool STAGED = LAYOUT >= ROWS_STAGED, GATES = LAYOUT == ROWS_GATES;
     // the row's place in its CTA, uniform over a warp
     const int ty = LAYOUT == ROWS_ONE ? 0 : __shfl_sync(0xffffffffu, int(threadIdx.y), 0), ny = LAYOUT == ROWS_ONE ? 1 : int(blockDim.y);
     constexpr int P = S::P;                                       // pairs of elements of a thread
@@ -271,8 +274,9 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
     const int K = p.K;
     const uint32_t slot_bytes = blockDim.x * V * 16;
     const uint32_t slot_x = smem_u32(smem) + ty * (rows_arrays(MODE) * slot_bytes), slot_h = slot_x + slot_bytes;
+    const int staged_words = S::staged_words(blockDim.x);
     float* const staged_pre = reinterpret_cast<float*>(smem + ny * (rows_arrays(MODE) * slot_bytes));
-    float* const staged_post = staged_pre + S::staged_words(blockDim.x);
+    float* const staged_post = staged_pre + staged_words;       // with the gate, or two of them with one gate each
     float2* const my_part = &part[0][0][0] + ty * (blockDim.x / 32);      // of [2][2]: this row's warps
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // One pass over the grid: the next kernel may set itself up meanwhile.  Not beside a persistent grid: CTAs that come early take
@@ -286,17 +290,20 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
         if (MODE == ROWS_BLOCK) S::fetch(row_of(p.h, p.ldh, row), K, shift, slot_h);
         S::fetch(row_of(p.x, p.ldx, row), K, shift, slot_x);
     };
-    const bool one_gate = p.gate && p.rows_per_gate >= p.M;
-    int row = blockIdx.x * ny + ty, turn = 0;
-    const int step = int(gridDim.x) * ny;
-    int shift = shift_of(row < p.M ? row : 0);
+    const bool staged_gate = STAGED && p.gate && (GATES || p.rows_per_gate >= p.M);
+    const int begin = int(blockIdx.x) * (GATES ? p.chunk : ny);
+    const int end = GATES && begin + p.chunk < p.M ? begin + p.chunk : p.M, step = GATES ? ny : int(gridDim.x) * ny;
+    const int first_gate = GATES ? begin / p.rows_per_gate : 0;
+    int row = begin + ty, turn = 0;
+    int shift = shift_of(row < end ? row : 0);
     S::clear(K, slot_x);
     if (MODE == ROWS_BLOCK) S::clear(K, slot_h);
-    if (row < p.M) fetch(row, shift);
+    if (row < end) fetch(row, shift);
     if constexpr (STAGED) {
         const uint16_t* w_pre = static_cast<const uint16_t*>(p.w_pre);
         const uint16_t* w_post = static_cast<const uint16_t*>(p.w_post);
-        const uint16_t* gate = static_cast<const uint16_t*>(p.gate);
+        const uint16_t* gate = static_cast<const uint16_t*>(p.gate) + int64_t(first_gate) * p.ldg;
+        const bool two = GATES && int64_t(first_gate + 1) * p.rows_per_gate < end;
         const int first = KIND == ROWS_SHIFTED ? -8 : 0, last = int(blockDim.x) * V * 8;
         for (int e = int(ty * blockDim.x + threadIdx.x) + first; e < last; e += int(blockDim.x) * ny) {
             const bool in = e >= 0 && e < K;
@@ -305,21 +312,22 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
             if (MODE == ROWS_BLOCK) {
                 float c = in ? 1.f : 0.f;
                 if (in && p.w_post) c = Pair<T>::lo(w_post[e]);
-                if (in && one_gate) c *= Pair<T>::lo(gate[e]);
+                if (two) staged_post[staged_words + at] = in ? c * Pair<T>::lo(gate[p.ldg + e]) : 0.f;
+                if (in && staged_gate) c *= Pair<T>::lo(gate[e]);
                 staged_post[at] = c;
             }
         }
         __syncthreads();
     }
-    while (row < p.M) {
-        const int next = row + step, next_shift = shift_of(next < p.M ? next : row);
+    while (row < end) {
+        const int next = row + step, next_shift = shift_of(next < end ? next : row);
         float2* const red = my_part + turn * 2 * (THREADS / 32);
         uint32_t x[P];
         float s = 0.f, m = 0.f;
         asm volatile("cp.async.wait_all;" ::: "memory");         // a thread reads only what it has fetched itself: no barrier
         S::take(slot_x, x);
         if constexpr (MODE == ROWS_QUANT) {
-            if (next < p.M) fetch(next, next_shift);
+            if (next < end) fetch(next, next_shift);
             uint32_t bits = 0;
 #pragma unroll
             for (int i = 0; i < P; i++) bits = __vmaxu2(bits, x[i] & 0x7fff7fffu);      // magnitudes order like their bits, NaN above all
@@ -338,7 +346,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
             if constexpr (MODE == ROWS_BLOCK) {
                 uint32_t h[P];
                 S::take(slot_h, h);
-                if (next < p.M) fetch(next, next_shift);
+                if (next < end) fetch(next, next_shift);
 #pragma unroll
                 for (int i = 0; i < P; i++) v[i] = up2<T>(h[i]);
                 if (p.w_post) {
@@ -349,12 +357,13 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
                     rstd = __frsqrt_rn(__fdiv_rn(s, float(K)) + p.eps);
                 }
                 const F2 rstd2 = f2(rstd, rstd), scale2 = f2(p.residual_scale, p.residual_scale);
-                const uint16_t* gate = p.gate && !(STAGED && one_gate) ? row_of(p.gate, p.ldg, row / p.rows_per_gate) : nullptr;
+                const float* const post = GATES && row >= (first_gate + 1) * p.rows_per_gate ? staged_post + staged_words : staged_post;
+                const uint16_t* gate = p.gate && !staged_gate ? row_of(p.gate, p.ldg, row / p.rows_per_gate) : nullptr;
 #pragma unroll
                 for (int g = 0; g < V; g++) {
                     F2 w[4];
                     if (STAGED || p.w_post) {
-                        if (STAGED) S::staged(staged_post, shift, g, w);
+                        if (STAGED) S::staged(post, shift, g, w);
                         else S::template peek<T>(p.w_post, K, shift, g, w);
 #pragma unroll
                         for (int i = 0; i < 4; i++) v[4 * g + i] = mul2(mul2(v[4 * g + i], rstd2), w[i]);
@@ -372,7 +381,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
                 }
                 S::store(const_cast<uint16_t*>(row_of(p.r, p.ldr, row)), K, shift, x);
             } else {
-                if (next < p.M) fetch(next, next_shift);
+                if (next < end) fetch(next, next_shift);
 #pragma unroll
                 for (int i = 0; i < P; i++) v[i] = up2<T>(x[i]);
             }
@@ -412,17 +421,22 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const RowsParams p) {
 // in flight on an SM.
 static bool rows_turn(const RowsParams& p) { return p.y && !p.codes && int64_t(p.M) * p.K * (p.h ? 8 : 4) > (int64_t(256) << 20); }
 
+template <int MODE, int V, int KIND, int LAYOUT>
+static int rows_smem(int threads, int groups) {
+    const int arrays = LAYOUT == ROWS_GATES ? 3 : (LAYOUT == ROWS_STAGED ? rows_arrays(MODE) : 0);       // of staged vectors
+    return groups * threads * V * 16 * rows_arrays(MODE) + Slots<V, KIND>::staged_words(threads) * 4 * arrays;
+}
+
 template <typename T, int MODE, int V, int KIND, int THREADS, int LAYOUT>
-static cudaError_t launch_rows_k(const RowsParams& p, int threads, int groups, int sm_count, cudaStream_t s) {
+static cudaError_t launch_rows_k(RowsParams p, int threads, int groups, int sm_count, cudaStream_t s) {
     auto kern = rows_kernel<T, MODE, V, KIND, THREADS, LAYOUT>;
-    const int staged = LAYOUT == ROWS_STAGED ? Slots<V, KIND>::staged_words(threads) * 4 * rows_arrays(MODE) : 0;
-    const int smem = groups * threads * V * 16 * rows_arrays(MODE) + staged;
+    const int smem = rows_smem<MODE, V, KIND, LAYOUT>(threads, groups);
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     static std::atomic<bool> attr_set[64] = {};
     if (!attr_set[dev].load(std::memory_order_acquire)) {
-        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024); e != cudaSuccess) return e;
+        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem); e != cudaSuccess) return e;
         attr_set[dev].store(true, std::memory_order_release);
     }
     // CTAs that an SM holds: asked for once for each device and size
@@ -440,7 +454,9 @@ static cudaError_t launch_rows_k(const RowsParams& p, int threads, int groups, i
         const int rows = 48 * 1024 / smem < 2 ? 2 : 48 * 1024 / smem;
         if (held > rows) held = rows;
     }
-    const int64_t fit = int64_t(sm_count) * held, want = (int64_t(p.M) + groups - 1) / groups;
+    const int64_t fit = int64_t(sm_count) * held;
+    if (LAYOUT == ROWS_GATES) p.chunk = int((p.M + fit - 1) / fit);
+    const int64_t want = LAYOUT == ROWS_GATES ? (int64_t(p.M) + p.chunk - 1) / p.chunk : (int64_t(p.M) + groups - 1) / groups;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(want < fit ? want : fit)); cfg.blockDim = dim3(threads, groups); cfg.dynamicSmemBytes = smem; cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -448,6 +464,17 @@ static cudaError_t launch_rows_k(const RowsParams& p, int threads, int groups, i
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+// Several gates are staged where sequences are no shorter than a CTA's rows (at most M / SMs), which then meet no more than two, and
+// there is room: gate rows read again and again against staged ones, in us: 4098 x 5001 with 6 gates 59.0 / 51.5, 16384 x 7168 with 8
+// 188 / 167, 8192 x 2048 with 16 38.4 / 26.6.
+template <typename T, int MODE, int V, int KIND, int THREADS>
+static cudaError_t launch_rows_staged(const RowsParams& p, int threads, int groups, int sm_count, cudaStream_t s) {
+    if constexpr (MODE == ROWS_BLOCK)
+        if (p.gate && p.rows_per_gate < p.M && p.rows_per_gate >= (p.M + sm_count - 1) / sm_count && rows_smem<MODE, V, KIND, ROWS_GATES>(threads, groups) <= kRowsSmem)
+            return launch_rows_k<T, MODE, V, KIND, THREADS, ROWS_GATES>(p, threads, groups, sm_count, s);
+    return launch_rows_k<T, MODE, V, KIND, THREADS, ROWS_STAGED>(p, threads, groups, sm_count, s);
 }
 
 // Few rows: as many threads for a row as it has groups of 8 elements (up to 1024), since the time from the first load to the last
@@ -467,12 +494,12 @@ static cudaError_t launch_rows_m(const RowsParams& p, int sm_count, cudaStream_t
             const int fit = most / threads(v) < 15 ? most / threads(v) : 15, turn = 64 * 1024 / (threads(v) * v * slot);
             return rows_turn(p) && turn < fit ? (turn < 1 ? 1 : turn) : fit;
         };
-        if (n8 <= 64) return launch_rows_k<T, MODE, 1, KIND, 768, ROWS_STAGED>(p, threads(1), rows(1, 768), sm_count, s);
+        if (n8 <= 64) return launch_rows_staged<T, MODE, 1, KIND, 768>(p, threads(1), rows(1, 768), sm_count, s);
         // Two groups for each thread rather than four shorten the way from load to store, where as many bytes stay in flight: rows of
         // which a CTA holds one either way (4096 x 16384 102.8 -> 96.5 us; 16384 x 8192 with int8 result, 2 rows rather than 3, 148 -> 164 us)
         if constexpr (KIND == ROWS_WHOLE)
-            if (n8 > 1536) return launch_rows_k<T, MODE, 2, KIND, 1024, ROWS_STAGED>(p, threads(2), 1, sm_count, s);
-        return launch_rows_k<T, MODE, 4, KIND, 768, ROWS_STAGED>(p, threads(4), rows(4, 768), sm_count, s);
+            if (n8 > 1536) return launch_rows_staged<T, MODE, 2, KIND, 1024>(p, threads(2), 1, sm_count, s);
+        return launch_rows_staged<T, MODE, 4, KIND, 768>(p, threads(4), rows(4, 768), sm_count, s);
     } else {
         if (n8 <= 64) return launch_rows_k<T, MODE, 2, KIND, 256, ROWS_WARPS>(p, 32, 8, sm_count, s);        // a warp for each row
         if (n8 <= 256) return launch_rows_k<T, MODE, 1, KIND, 256, ROWS_ONE>(p, threads(1), 1, sm_count, s);
