@@ -496,10 +496,13 @@ static cudaError_t launch_rows_m(const RowsParams& p, int sm_count, cudaStream_t
         };
         if (n8 <= 64) return launch_rows_staged<T, MODE, 1, KIND, 768>(p, threads(1), rows(1, 768), sm_count, s);
         // Two groups for each thread rather than four shorten the way from load to store, where as many bytes stay in flight: rows of
-        // which a CTA holds one either way (4096 x 16384 102.8 -> 96.5 us; 16384 x 8192 with int8 result, 2 rows rather than 3, 148 -> 164 us)
-        if constexpr (KIND == ROWS_WHOLE)
-            if (n8 > 1536) return launch_rows_staged<T, MODE, 2, KIND, 1024>(p, threads(2), 1, sm_count, s);
-        return launch_rows_staged<T, MODE, 4, KIND, 768>(p, threads(4), rows(4, 768), sm_count, s);
+        // which a CTA holds one either way (4096 x 16384 102.8 -> 96.5 us; 16384 x 8192 with int8 result, 2 rows rather than 3, 148 -> 164
+        // us); short shifted rows, of which four groups would make one or two warps (8190 x 1001 28.2 -> 24.2 us, 8190 x 1501 36.3 -> 32.5,
+        // 4090 x 3001 30.7 -> 33.6); single elements, whose addresses do not fit the registers of four groups (4098 x 5001 136 -> 104 us)
+        if (KIND == ROWS_SINGLE || n8 > 1536 || (KIND == ROWS_SHIFTED && n8 <= 192))
+            return launch_rows_staged<T, MODE, 2, KIND, 1024>(p, threads(2), rows(2, 1024), sm_count, s);
+        if constexpr (KIND != ROWS_SINGLE) return launch_rows_staged<T, MODE, 4, KIND, 768>(p, threads(4), rows(4, 768), sm_count, s);
+        return cudaErrorInvalidValue;
     } else {
         if (n8 <= 64) return launch_rows_k<T, MODE, 2, KIND, 256, ROWS_WARPS>(p, 32, 8, sm_count, s);        // a warp for each row
         if (n8 <= 256) return launch_rows_k<T, MODE, 1, KIND, 256, ROWS_ONE>(p, threads(1), 1, sm_count, s);
