@@ -352,7 +352,10 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
         if (overlap(out, s)) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: D overlaps %s", s.name);
     DeviceCtx* c;
     if (int e = get_ctx(&c)) return e;
-    if (M <= kInt8SkinnyMaxM && config == TKB_GEMM_DEFAULT) {
+    // few tokens; over 64 of them with a short K rather as one wave of tiles (128 tokens, streamed / tiles: N=2048 K=512 5.7 / 4.3 us, N=8192
+    // K=1024 7.5 / 7.0 us, N=7168 K=2048 9.1 / 9.0 us)
+    const bool short_k = K <= 1024;
+    if (M <= kInt8SkinnyMaxM && config == TKB_GEMM_DEFAULT && !(M > 64 && short_k && (N + 127) / 128 <= c->sm_count)) {
         SkinnyArgs a;
         memset(&a, 0, sizeof(a));
         if (!int8_skinny_short(M, N, c->sm_count)) {
@@ -370,12 +373,14 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
     g.kind = KIND_INT8;
     g.config = pick_config(KIND_INT8, config, M, N, c->sm_count);
     // short K: the epilogue counts for more than the loads that a CTA pair saves (M=N=8192, pairs / single CTAs: K=512 48.6 / 41.8 us, K=1024
-    // 60.4 / 60.5 us, K=2048 94.2 / 103.5 us)
-    if (config == TKB_GEMM_DEFAULT && K < 1024) g.config |= 1;
-    // one wave of 128 x 128 tiles rather than two of CTA pairs: M=333 N=5000 K=4112 17.9 us against 24.0 us
-    if (config == TKB_GEMM_DEFAULT && g.config == 2 && long((M + 255) / 256) * ((N + 127) / 128) * 2 > c->sm_count &&
-        long((M + 127) / 128) * ((N + 127) / 128) <= c->sm_count)
-        g.config = 3;
+    // 60.4 / 60.5 us, K=2048 94.2 / 103.5 us; M=1024 N=1024 K=1024 6.3 / 5.6 us)
+    if (config == TKB_GEMM_DEFAULT && short_k) g.config |= 1;
+    // one wave of 128 x 128 tiles, or of pairs with 256 x 256 tiles, rather than two of pairs with 256 x 128: M=333 N=5000 K=4112 17.9 us against
+    // 24.0 us; M=700 N=5001 K=4112 21.4 against 25.7, M=4096 N=1000 K=8192 25.4 against 29.4
+    if (config == TKB_GEMM_DEFAULT && g.config == 2 && long((M + 255) / 256) * ((N + 127) / 128) * 2 > c->sm_count) {
+        if (long((M + 127) / 128) * ((N + 127) / 128) <= c->sm_count) g.config = 3;
+        else if (long((M + 255) / 256) * ((N + 255) / 256) * 2 <= c->sm_count) g.config = 0;
+    }
     const int ctas = (g.config & 1) ? 1 : 2;
     if (int e = make_operand_map(&g.tmA, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, lda, 128)) return e;
     if (int e = make_operand_map(&g.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, ldb, gemm_tile_n(g.config) / ctas)) return e;
