@@ -352,10 +352,9 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
         if (overlap(out, s)) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: D overlaps %s", s.name);
     DeviceCtx* c;
     if (int e = get_ctx(&c)) return e;
-    // few tokens; over 64 of them with a short K rather as one wave of tiles (128 tokens, streamed / tiles: N=2048 K=512 5.7 / 4.3 us, N=8192
-    // K=1024 7.5 / 7.0 us, N=7168 K=2048 9.1 / 9.0 us)
-    const bool short_k = K <= 1024;
-    if (M <= kInt8SkinnyMaxM && config == TKB_GEMM_DEFAULT && !(M > 64 && short_k && (N + 127) / 128 <= c->sm_count)) {
+    // few tokens; over 64 of them with a short K rather as tiles, few of them or for the shortest K (128 tokens, streamed / tiles: N=2048 K=512
+    // 5.7 / 4.3 us, N=7168 K=2048 9.2 / 8.2 us, N=28672 K=512 11.3 / 7.7 us; N=50257 K=1024 17.1 / 18.2 us, N=2048 K=7168 14.7 / 15.4 us)
+    if (M <= kInt8SkinnyMaxM && config == TKB_GEMM_DEFAULT && !(M > 64 && (K <= 512 || (K <= 2048 && (N + 127) / 128 <= c->sm_count)))) {
         SkinnyArgs a;
         memset(&a, 0, sizeof(a));
         if (!int8_skinny_short(M, N, c->sm_count)) {
@@ -372,9 +371,13 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
     memset(&g, 0, sizeof(g));
     g.kind = KIND_INT8;
     g.config = pick_config(KIND_INT8, config, M, N, c->sm_count);
-    // short K: the epilogue counts for more than the loads that a CTA pair saves (M=N=8192, pairs / single CTAs: K=512 48.6 / 41.8 us, K=1024
-    // 60.4 / 60.5 us, K=2048 94.2 / 103.5 us; M=1024 N=1024 K=1024 6.3 / 5.6 us)
-    if (config == TKB_GEMM_DEFAULT && short_k) g.config |= 1;
+    // short K: the way through one tile counts for more than the loads that a CTA pair saves.  Up to two waves of 128 x 128 tiles: M=N=K=1024
+    // 5.9 (pairs, 256 x 128) / 5.6 us, M=512 N=8192 K=512 7.8 (pairs, 256 x 256) / 6.6 us, M=4096 N=1024 K=1024 9.3 / 8.6 us.  More, and less than
+    // four blocks of K, 128 x 256 tiles: M=2048 N=4096 K=256 8.3 (pairs) / 7.8 us, but M=N=8192 K=512 38.3 / 41.7 us
+    if (config == TKB_GEMM_DEFAULT && (K <= 1024 || M <= 128)) {
+        if (g.config == 2 || M <= 128 || long((M + 127) / 128) * ((N + 127) / 128) <= 2 * c->sm_count) g.config = 3;
+        else if (K < 512) g.config = 1;
+    }
     // one wave of 128 x 128 tiles, or of pairs with 256 x 256 tiles, rather than two of pairs with 256 x 128: M=333 N=5000 K=4112 17.9 us against
     // 24.0 us; M=700 N=5001 K=4112 21.4 against 25.7, M=4096 N=1000 K=8192 25.4 against 29.4
     if (config == TKB_GEMM_DEFAULT && g.config == 2 && long((M + 255) / 256) * ((N + 127) / 128) * 2 > c->sm_count) {

@@ -130,11 +130,13 @@ __device__ __forceinline__ uint8_t quant_block16(const uint32_t (&w)[8], float s
 // Epilogue of KIND_INT8 for one warp: 32 rows x 64 columns of int32 sums (this thread: row row0 + lane) from tensor memory are scaled,
 // converted and leave through the warp's staging box (rows of 128 bytes, 128-byte swizzle): one box of 64 columns for the 16-bit
 // types, two of 32 columns for fp32.  The sums are converted to fp32 first (one rounding above 2^24), then multiplied by the row's
-// and by the column's scale.  A box leaves by TMA, which clips the edges of D, or (DIRECT), where D's base or pitch is not a multiple
-// of 16 bytes, row by row with one element per lane.
-template <bool DIRECT>
+// and by the column's scale.  The warp's lanes hold the scales of its columns, NV in each, from `first_lane` on for these 64: with L1
+// given to the operands a load here would be one from L2.  A box leaves by TMA, which clips the edges of D, or (DIRECT), where D's base or
+// pitch is not a multiple of 16 bytes, row by row with one element per lane (words of two 16-bit values, whose odd rows leave one value
+// at each end, took 139 us for 8192 x 8191 x 1024 where this takes 75).
+template <bool DIRECT, int NV>
 __device__ __forceinline__ void int8_epilogue(uint32_t acc_t, const CUtensorMap* tmD, const GemmParams& p, uint32_t stage_box, int row0, int col0,
-                                              float row_scale, int lane, uint64_t policy) {
+                                              float row_scale, const float (&col_scale)[NV], int first_lane, int lane, uint64_t policy) {
     if (row0 >= p.M || col0 >= p.N) return;                  // uniform over the warp
     auto leave = [&](int col, int elem_bytes) {              // the box holds columns col .. col + 128 / elem_bytes - 1
         if constexpr (!DIRECT) {
@@ -148,28 +150,30 @@ __device__ __forceinline__ void int8_epilogue(uint32_t acc_t, const CUtensorMap*
         }
         __syncwarp();
         // 8 rows at a time, so that their loads and stores are in flight together
-        const int rows = min(32, p.M - row0);
-        const bool in0 = col + lane < p.N, in1 = col + lane + 32 < p.N;
-        for (int row = 0; row < rows; row += 8) {
-            uint32_t v[8][2];
+        const int rows = min(32, p.M - row0), left = p.N - col;
+        constexpr int HALVES = 2;                            // of a row of 16-bit values; an fp32 row has 32
+        const int64_t pitch = p.ldd * elem_bytes;
+        char* out = static_cast<char*>(p.D) + (int64_t(row0) * p.ldd + col + lane) * elem_bytes;
+        for (int row = 0; row < rows; row += 8, out += 8 * pitch) {
+            uint32_t v[8][HALVES];
 #pragma unroll
             for (int k = 0; k < 8; k++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < HALVES; h++) {
                     const uint32_t at = uint32_t(lane + 32 * h) * elem_bytes;
-                    const uint32_t src = stage_box + (row + k) * 128 + ((((at >> 4) & 7u) ^ uint32_t((row + k) & 7)) << 4) + (at & 15u);
+                    const uint32_t src = stage_box + (row + k) * 128 + ((((at >> 4) & 7u) ^ uint32_t(k)) << 4) + (at & 15u);
                     if (elem_bytes == 2) { uint16_t u; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(src) : "memory"); v[k][h] = u; }
-                    else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[k][h]) : "r"(src) : "memory");
+                    else if (h == 0) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[k][h]) : "r"(src) : "memory");
                 }
+            char* to = out;
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                if (row + k >= rows) continue;
-                const int64_t at = int64_t(row0 + row + k) * p.ldd + col + lane;
+            for (int k = 0; k < 8; k++, to += pitch) {
+                if (row + k >= rows) break;
                 if (elem_bytes == 2) {
-                    if (in0) static_cast<uint16_t*>(p.D)[at] = uint16_t(v[k][0]);
-                    if (in1) static_cast<uint16_t*>(p.D)[at + 32] = uint16_t(v[k][1]);
-                } else if (in0) {                            // (an fp32 box has 32 columns)
-                    static_cast<uint32_t*>(p.D)[at] = v[k][0];
+                    if (lane < left) *reinterpret_cast<uint16_t*>(to) = uint16_t(v[k][0]);
+                    if (lane + 32 < left) *reinterpret_cast<uint16_t*>(to + 64) = uint16_t(v[k][1]);
+                } else if (lane < left) {
+                    *reinterpret_cast<uint32_t*>(to) = v[k][0];
                 }
             }
         }
@@ -188,19 +192,10 @@ __device__ __forceinline__ void int8_epilogue(uint32_t acc_t, const CUtensorMap*
         __syncwarp();
         tmem_ld_32x32(acc_t + 32 * h, r);
         tmem_ld_wait();
-        const float* cs = p.sgB + col;
-        if (col + 32 <= p.N && (reinterpret_cast<uintptr_t>(cs) & 15u) == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float4 c = reinterpret_cast<const float4*>(cs)[i];      // the same address in all lanes
-                r[4 * i] = __float_as_uint(__int2float_rn(int(r[4 * i])) * row_scale * c.x);
-                r[4 * i + 1] = __float_as_uint(__int2float_rn(int(r[4 * i + 1])) * row_scale * c.y);
-                r[4 * i + 2] = __float_as_uint(__int2float_rn(int(r[4 * i + 2])) * row_scale * c.z);
-                r[4 * i + 3] = __float_as_uint(__int2float_rn(int(r[4 * i + 3])) * row_scale * c.w);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; i++) r[i] = __float_as_uint(__int2float_rn(int(r[i])) * row_scale * p.sgB[min(col + i, p.N - 1)]);
+        for (int i = 0; i < 32; i++) {
+            const float c = __shfl_sync(0xffffffffu, col_scale[i % NV], first_lane + (32 * h + i) / NV);
+            r[i] = __float_as_uint(__int2float_rn(int(r[i])) * row_scale * c);
         }
         if (fp32) {
             box_free();
@@ -807,15 +802,27 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         uint32_t tile_count = 0;
         bool ok = true;
         long long wait_tf = 0, drain = 0;
+        // KIND_INT8: the scale of the thread's row and its share of the warp's columns, for the next tile (zeros outside of D)
+        constexpr int NV = C::COLS_PER_EPI_WARP / 32;
+        float next_row_scale = 0.f, next_col_scale[NV] = {};
+        auto load_scales = [&](int tile) {
+            int m_blk, n_blk;
+            tile_to_block(tile, tiles_m, tiles_n, tile_group, tile_rot, m_blk, n_blk);
+            const int row = m_blk * C::BM + int(cta_rank) * 128 + quarter * 32 + lane, col = n_blk * BN + col_base + lane * NV;
+            next_row_scale = row < p.M ? p.sgA[row] : 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; j++) next_col_scale[j] = col + j < p.N ? p.sgB[col + j] : 0.f;
+        };
+        if (KIND == KIND_INT8 && first_tile < num_tiles) load_scales(first_tile);
         for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride) {
             int m_blk, n_blk;
             tile_to_block(tile, tiles_m, tiles_n, tile_group, tile_rot, m_blk, n_blk);
-            float row_scale = 0.f;       // (a row that TMA clips or the plain stores leave out)
-            if constexpr (KIND == KIND_INT8) {
-                const int row = m_blk * C::BM + int(cta_rank) * 128 + quarter * 32 + lane;
-                if (row < p.M) row_scale = p.sgA[row];
-            }
-            (void)row_scale;
+            const float row_scale = next_row_scale;
+            float col_scale[NV];
+#pragma unroll
+            for (int j = 0; j < NV; j++) col_scale[j] = next_col_scale[j];
+            if (KIND == KIND_INT8 && tile + tile_stride < num_tiles) load_scales(tile + tile_stride);
+            (void)row_scale; (void)col_scale;
             const long long t0 = clock64();
             const uint32_t buf = tile_count % C::ACC_BUFS;
             if (!mbar_wait(wc, smem_u32(&bar_tmem_full[buf]), (tile_count / C::ACC_BUFS) & 1u)) { ok = false; break; }
@@ -827,14 +834,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                 const int row0 = m_blk * C::BM + int(cta_rank) * 128 + quarter * 32;
                 const int col0 = n_blk * BN + col_base;
                 const uint32_t acc_t = tmem_base + (uint32_t(quarter * 32) << 16) + buf * C::ACC_COLS + col_base;
-                int8_epilogue<MODE == MODE_DIRECT>(acc_t, &tmD, p, stage_box, row0, col0, row_scale, lane, d_policy);
+                int8_epilogue<MODE == MODE_DIRECT>(acc_t, &tmD, p, stage_box, row0, col0, row_scale, col_scale, 0, lane, d_policy);
                 if (C::COLS_PER_EPI_WARP > 64)
-                    int8_epilogue<MODE == MODE_DIRECT>(acc_t + 64, &tmD, p, stage_box, row0, col0 + 64, row_scale, lane, d_policy);
+                    int8_epilogue<MODE == MODE_DIRECT>(acc_t + 64, &tmD, p, stage_box, row0, col0 + 64, row_scale, col_scale, 64 / NV, lane, d_policy);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {                             // (two accumulators: the next tile's MMAs are under way)
                     const uint32_t tmem_empty_leader = buf ? tmem_empty_leader1 : tmem_empty_leader0;
-                    if constexpr (CTAS == 2) mbar_arrive_cluster(tmem_empty_leader); else mbar_arrive(tmem_empty_leader);
+                    if constexpr (CTAS == 2) mbar_arrive_cluster_tmem(tmem_empty_leader); else mbar_arrive(tmem_empty_leader);
                 }
                 drain += clock64() - t1;
                 continue;
