@@ -111,6 +111,17 @@ def test_gemm(cuda, lib, M, N, K, out):
     _check_gemm(D, a, a_sc, b, b_sc)
 
 
+@pytest.mark.parametrize("M", [9, 33, 48, 49, 70, 90, 110, 128])
+@pytest.mark.parametrize("N,K", [(333, 2100), (5000, 2176), (9001, 2300), (19000, 2064), (40000, 2100)])
+def test_gemm_streamed_weights(cuda, lib, M, N, K):
+    """Few tokens: every padding of them, slabs of few and of many weight rows, K that ends inside a stage and inside a block."""
+    a, a_sc, b, b_sc = _operands(M, N, K, cuda, seed=5)
+    for out in (torch.float16, torch.float32):
+        D = torch.full((M, N), float("nan"), dtype=out, device=cuda)
+        _ops().int8_gemm(a, a_sc, b, b_sc, D)
+        _check_gemm(D, a, a_sc, b, b_sc)
+
+
 @pytest.mark.parametrize("cfg", ["pair_n256", "single_n256", "pair_n128", "single_n128"])
 @pytest.mark.parametrize("M,N,K", [(1, 40, 48), (130, 264, 272), (600, 513, 900), (2048, 1536, 1024)])
 def test_gemm_tiles(cuda, lib, M, N, K, cfg):
@@ -283,3 +294,17 @@ def test_refusals_on_tensors(cuda, lib):
         with pytest.raises(RuntimeError, match=word):
             ops.int8_quantize(*args)
     assert float(D.abs().sum()) == 0.0
+
+
+def test_numbers_that_are_none(cuda, lib):
+    """What is no number is refused by name; numbers of any Python type are taken."""
+    ops = _ops()
+    x, w, Y = torch.ones(4, 64, dtype=torch.bfloat16, device=cuda), torch.ones(64, dtype=torch.bfloat16, device=cuda), torch.empty(4, 64, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(RuntimeError, match="eps"):
+        ops.rms_norm(x, w, Y, eps="small")
+    with pytest.raises(RuntimeError, match="residual_scale"):
+        ops.block_norm(x, x, Y, residual_scale=None)
+    ops.block_norm(H=x, X=x, X_out=Y, residual_scale=2, eps=1)
+    assert bool((Y == 3).all())
+    with pytest.raises(RuntimeError, match="must be a torch.Tensor"):
+        ops.rms_norm(x, [1.0] * 64, Y)
