@@ -228,7 +228,7 @@ int tkb_fp8_gemm_ex(const void* A, int64_t lda, const void* B, int64_t ldb, void
  *   Any M >= 0, N >= 1, 1 <= K <= 131071 (the sum is exact in int32), odd ones too; M, N <= 2^30.  The sum is converted to fp32,
  *   multiplied by A_sc[m], then by B_sc[n], and rounded to `dtype`: results depend neither on the run nor on the kernel or tile that
  *   the sizes choose.  D may not overlap the operands.  No scratch: calls on any streams and captured graphs are independent.
- * Up to 128 tokens stream the weights once (one of two kernels, by N; over 64 with a short K not); others go through the GEMM tiles.  The _ex form takes
+ * Up to 128 tokens stream the weights once (one of two kernels, by N; over 64 with a short K or few outputs not); others go through the GEMM tiles.  The _ex form takes
  * TKB_GEMM_PAIR_N256 .. TKB_GEMM_SINGLE_N128 for any M.  No counterpart in the reference. */
 int tkb_int8_gemm(const void* A, int64_t lda, const float* A_sc, const void* B, int64_t ldb, const float* B_sc, void* D, int64_t ldd, int dtype,
                   int M, int N, int K, void* stream);

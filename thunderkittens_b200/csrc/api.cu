@@ -352,9 +352,9 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
         if (overlap(out, s)) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: D overlaps %s", s.name);
     DeviceCtx* c;
     if (int e = get_ctx(&c)) return e;
-    // few tokens; over 64 of them with a short K rather as tiles, few of them or for the shortest K (128 tokens, streamed / tiles: N=2048 K=512
+    // few tokens; over 64 of them rather as tiles where one wave of 128 x 64 holds them or K is short (128 tokens, streamed / tiles: N=2048 K=512
     // 5.7 / 4.3 us, N=7168 K=2048 9.2 / 8.2 us, N=28672 K=512 11.3 / 7.7 us; N=50257 K=1024 17.1 / 18.2 us, N=2048 K=7168 14.7 / 15.4 us)
-    if (M <= kInt8SkinnyMaxM && config == TKB_GEMM_DEFAULT && !(M > 64 && (K <= 512 || (K <= 2048 && (N + 127) / 128 <= c->sm_count)))) {
+    if (M <= kInt8SkinnyMaxM && config == TKB_GEMM_DEFAULT && !(M > 64 && (K <= 512 || N <= 64 * c->sm_count || (K <= 2048 && N <= 128 * c->sm_count)))) {
         SkinnyArgs a;
         memset(&a, 0, sizeof(a));
         if (!int8_skinny_short(M, N, c->sm_count)) {
@@ -384,6 +384,9 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
         if (long((M + 127) / 128) * ((N + 127) / 128) <= c->sm_count) g.config = 3;
         else if (long((M + 255) / 256) * ((N + 255) / 256) * 2 <= c->sm_count) g.config = 0;
     }
+    // 128 x 64 tiles where they are no more than SMs (256 x 128 of a pair / these: M=256 N=1000 K=8192 15.7 / 13.5 us, N=K=4096 10.5 / 9.3 us; 128 x 128
+    // / these: M=N=K=1024 5.6 / 4.7 us; 80 tokens streamed / these: N=2048 K=7168 12.4 / 12.2 us, N=K=4096 10.0 / 9.1 us)
+    if (config == TKB_GEMM_DEFAULT && long((M + 127) / 128) * ((N + 63) / 64) <= c->sm_count) g.config = 9;
     const int ctas = (g.config & 1) ? 1 : 2;
     if (int e = make_operand_map(&g.tmA, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, M, lda, 128)) return e;
     if (int e = make_operand_map(&g.tmB, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, N, ldb, gemm_tile_n(g.config) / ctas)) return e;

@@ -44,7 +44,7 @@ namespace tkb {
 template <int KIND, int CTAS, int BN, int MH = 1>
 struct GemmCfg {
     static_assert(CTAS == 1 || CTAS == 2, "");
-    static_assert(BN == 128 || BN == 256, "");
+    static_assert(BN == 128 || BN == 256 || (BN == 64 && KIND == KIND_INT8), "");
     // MH = 2 (dense kinds, CTA pairs, N tile 256): every CTA carries TWO 128-row halves of A per stage against the same B rows,
     // i.e. a 512 x 256 cluster tile with one accumulator per half: a third more FLOPs per byte that crosses from L2 into
     // shared memory than the 256 x 256 tile, which is what bounds the dense kernels
@@ -52,14 +52,17 @@ struct GemmCfg {
     static constexpr int BM = 128 * CTAS * MH;            // rows of D per cluster tile
     static constexpr int MMA_M = 128 * CTAS;              // rows of one MMA instruction (per CTA pair)
     static constexpr int BN_CTA = BN / CTAS;              // rows of B each CTA loads
-    static constexpr int KB = KIND == KIND_BF16 ? 64 : (KIND == KIND_NVFP4 ? 256 : 128);   // K elements per stage (128 bytes)
-    static constexpr int A_BYTES = MH * 128 * 128;
-    static constexpr int B_BYTES = BN_CTA * 128;
+    // blocks of 128 bytes of K in a stage: two for N tile 64, where the loops of the two threads that feed it take longer than one (M=129
+    // N=200 K=8192 13.5 us with one, 10.8 with two); past the end of K the second loads zeros
+    static constexpr int GROUP = BN == 64 ? 2 : 1;
+    static constexpr int KB = GROUP * (KIND == KIND_BF16 ? 64 : (KIND == KIND_NVFP4 ? 256 : 128));   // K elements per stage
+    static constexpr int A_BYTES = GROUP * MH * 128 * 128;
+    static constexpr int B_BYTES = GROUP * BN_CTA * 128;
     static constexpr int SF_CHUNKS = KIND == KIND_NVFP4 ? 4 : (KIND == KIND_MXFP8 ? 1 : 0);  // 512-byte chunks per 128 rows per stage
     static constexpr int SFA_BYTES = SF_CHUNKS * 512;
     static constexpr int SFB_BYTES = SF_CHUNKS * 512 * (BN / 128);
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
-    static constexpr int EPI_WARPS = BN == 256 || KIND == KIND_INT8 ? 8 : 4;
+    static constexpr int EPI_WARPS = BN == 256 || (KIND == KIND_INT8 && BN == 128) ? 8 : 4;
     static constexpr int EPI_WARP_BYTES = 32 * 128;                  // one 32-row x 64-column bf16 store box per warp
     static constexpr int EPI_BYTES = EPI_WARPS * EPI_WARP_BYTES;
     static constexpr int SMEM_BUDGET = 227 * 1024 - 2048 - EPI_BYTES;
@@ -664,7 +667,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                       waited += clock64() - t0; }
                     const uint32_t full_local = smem_u32(&bar_full[stage]);
                     if (is_leader) mbar_arrive_expect_tx(full_local, C::TX_BYTES);
-                    const int kx = kb * 128 / (KIND == KIND_BF16 ? 2 : 1);   // inner coordinate in tensor-map elements (bf16 or bytes)
+                    const int kx = kb * C::GROUP * 128 / (KIND == KIND_BF16 ? 2 : 1);   // inner coordinate in tensor-map elements (bf16 or bytes)
                     if constexpr (CTAS == 2) {
                         const uint32_t full = mapa(full_local, 0);
                         tma_load_2d_pair(sA + stage * C::A_BYTES, &tmA, full, kx, a_row);
@@ -677,8 +680,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                                                  b_sblk + j);
                         }
                     } else {
-                        tma_load_2d(sA + stage * C::A_BYTES, &tmA, full_local, kx, a_row);
-                        tma_load_2d(sB + stage * C::B_BYTES, &tmB, full_local, kx, b_row);
+#pragma unroll
+                        for (int g = 0; g < C::GROUP; g++) {
+                            tma_load_2d(sA + stage * C::A_BYTES + g * 128 * 128, &tmA, full_local, kx + g * 128, a_row);
+                            tma_load_2d(sB + stage * C::B_BYTES + g * BN * 128, &tmB, full_local, kx + g * 128, b_row);
+                        }
                         if constexpr (SCALED) {
                             tma_load_3d(sSA + stage * C::SFA_BYTES, &tmSA, full_local, 0, kb * C::SF_CHUNKS, m_blk);
 #pragma unroll
@@ -756,6 +762,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
                                 mma_f8<CTAS>(acc_h, a_desc + 2 * j, b_desc + 2 * j, idesc_fp8(C::MMA_M, BN), acc);
                             } else if constexpr (KIND == KIND_INT8) {
                                 mma_i8<CTAS>(acc_h, a_desc + 2 * j, b_desc + 2 * j, idesc_int8(C::MMA_M, BN), acc);
+                                if constexpr (C::GROUP == 2) {
+                                    if (j == 3)
+#pragma unroll
+                                        for (int i = 0; i < 4; i++)
+                                            mma_i8<CTAS>(acc_h, a_desc + 128 * 128 / 16 + 2 * i, b_desc + BN * 128 / 16 + 2 * i, idesc_int8(C::MMA_M, BN), 1u);
+                                }
                             } else if constexpr (KIND == KIND_MXFP8) {
                                 mma_mxfp8<CTAS>(acc_h, a_desc + 2 * j, b_desc + 2 * j, idesc_mxfp8(C::MMA_M, BN, j), acc, sfa_t, sfb_t);
                             } else {
@@ -1037,6 +1049,9 @@ static cudaError_t launch_k(const GemmArgs& a) {
     if constexpr (KIND == KIND_BF16 || KIND == KIND_FP8) {
         if (a.config & 4) return launch_t<KIND, 2, 256, MODE_PLAIN, 2>(a);      // 512 x 256 cluster tiles
     }
+    if constexpr (KIND == KIND_INT8) {
+        if (a.config & 8) return launch_t<KIND, 1, 64, MODE>(a);
+    }
     switch (a.config & 3) {
         case 0: return launch_t<KIND, 2, 256, MODE>(a);
         case 1: return launch_t<KIND, 1, 256, MODE>(a);
@@ -1054,7 +1069,7 @@ int moe_dispatch_ring(int K) {
     return int(ring < 0 ? 0 : (ring > 32 ? 32 : ring));
 }
 
-int gemm_tile_n(int config) { return (config & 2) ? 128 : 256; }
+int gemm_tile_n(int config) { return (config & 8) ? 64 : ((config & 2) ? 128 : 256); }
 int gemm_tile_m(int config) { return (config & 4) ? 512 : ((config & 1) ? 128 : 256); }
 
 cudaError_t launch_gemm(const GemmArgs& a) {

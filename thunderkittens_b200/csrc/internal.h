@@ -63,7 +63,7 @@ struct CommParams { AgParams ag; MoeParams moe; };
 
 struct GemmArgs {
     int kind;                 // GemmKind
-    int config;               // bit 0: 0 = CTA pair (cta_group::2), 1 = single CTA; bit 1: 0 = N tile 256, 1 = N tile 128
+    int config;               // bit 0: 0 = CTA pair (cta_group::2), 1 = single CTA; bit 1: 0 = N tile 256, 1 = N tile 128; bit 3: N tile 64 (KIND_INT8, single CTA)
     CUtensorMap tmA, tmB, tmSA, tmSB, tmD;   // tmD: bf16 output, box 64 columns x 32 rows, 128-byte swizzle
     const float* sgA; const float* sgB;
     int M, N, K;
