@@ -144,7 +144,8 @@ int tkb_int8_quantize(const void* A, int64_t lda, int dtype, void* codes, int64_
  *   X, Y [M, K], W [K], all of `dtype` (bf16 or fp16); row pitches in elements (0 = K).  0 <= M <= 2^30, 1 <= K <= 16384, any
  *   alignment (16-byte aligned rows and K % 8 == 0 go fastest, next rows of all tensors that begin alike within 16 bytes).  Sums and
  *   y are held in fp32: |x| above about 1e19 overflows its square.  Outputs may not overlap an input or one another.  Y and the
- *   codes are the same whether one or both are asked for.
+ *   codes are the same whether one or both are asked for, as long as the tensor that comes along does not change the alignment just named
+ *   (which decides how a row is dealt out to threads, and with that the order of its sums).
  * No counterpart in the reference. */
 int tkb_rms_norm(const void* X, int64_t ldx, const void* W, void* Y, int64_t ldy, void* codes, int64_t ldc, float* sc, int dtype, int M, int K,
                  float eps, void* stream);
@@ -155,7 +156,7 @@ int tkb_rms_norm(const void* X, int64_t ldx, const void* W, void* Y, int64_t ldy
  *   y = r * rsqrt(mean_k r^2 + eps) * W_pre      (left out if W_pre is NULL)    -> Y and / or codes, sc as in tkb_rms_norm
  *   H (the block's output), X (the residual stream), R, Y [M, K], W_post, W_pre [K] and gate of `dtype`; row i uses gate row
  *   i / rows_per_gate of pitch ldg: one gate for all (rows_per_gate >= M), one for each sequence of a batch, one for each token.
- *   y is made from the unrounded r.  R may be X itself (same pointer and pitch); otherwise outputs may not overlap an input or one
+ *   y is made from the unrounded r.  R, Y and the codes are the same whichever are asked for, as in tkb_rms_norm.  R may be X itself (same pointer and pitch); otherwise outputs may not overlap an input or one
  *   another.  residual_scale is a finite number.  Sizes, pitches and precision as in tkb_rms_norm.
  * No counterpart in the reference. */
 int tkb_block_norm(const void* H, int64_t ldh, const void* X, int64_t ldx, void* R, int64_t ldr, const void* W_post, const void* gate, int64_t ldg,

@@ -467,12 +467,17 @@ static cudaError_t launch_rows_k(RowsParams p, int threads, int groups, int sm_c
 }
 
 // Several gates are staged where sequences are no shorter than a CTA's rows (at most M / SMs), which then meet no more than two, and
-// there is room: gate rows read again and again against staged ones, in us: 4098 x 5001 with 6 gates 59.0 / 51.5, 16384 x 7168 with 8
-// 188 / 167, 8192 x 2048 with 16 38.4 / 26.6.
+// there is room beside as many rows as a CTA may have: gate rows read again and again against staged ones, in us: 4098 x 5001 with 6
+// gates 59.0 / 51.5, 16384 x 7168 with 8 188 / 167, 8192 x 2048 with 16 38.4 / 26.6.  Where only fewer rows leave the room, rows count for
+// more: 4096 x 12288 with 2, int8 result, 80 / 99.  The two round apart (one multiplies by the product w_post * gate, the other by one after
+// the other), so the choice may not depend on which results are asked for, as the rows of a CTA do (rows_turn).
 template <typename T, int MODE, int V, int KIND, int THREADS>
-static cudaError_t launch_rows_staged(const RowsParams& p, int threads, int groups, int sm_count, cudaStream_t s) {
+static cudaError_t launch_rows_staged(const RowsParams& p, int threads, int most, int sm_count, cudaStream_t s) {
+    const int fit = most / threads < 15 ? most / threads : 15;                  // rows of a CTA (15: as many as it has barriers)
+    const int turn = 64 * 1024 / (threads * V * 16 * rows_arrays(MODE));
+    const int groups = rows_turn(p) && turn < fit ? (turn < 1 ? 1 : turn) : fit;
     if constexpr (MODE == ROWS_BLOCK)
-        if (p.gate && p.rows_per_gate < p.M && p.rows_per_gate >= (p.M + sm_count - 1) / sm_count && rows_smem<MODE, V, KIND, ROWS_GATES>(threads, groups) <= kRowsSmem)
+        if (p.gate && p.rows_per_gate < p.M && p.rows_per_gate >= (p.M + sm_count - 1) / sm_count && rows_smem<MODE, V, KIND, ROWS_GATES>(threads, fit) <= kRowsSmem)
             return launch_rows_k<T, MODE, V, KIND, THREADS, ROWS_GATES>(p, threads, groups, sm_count, s);
     return launch_rows_k<T, MODE, V, KIND, THREADS, ROWS_STAGED>(p, threads, groups, sm_count, s);
 }
@@ -489,19 +494,14 @@ static cudaError_t launch_rows_m(const RowsParams& p, int sm_count, cudaStream_t
     if (p.M <= 2 * sm_count && n8 <= 1024) return launch_rows_k<T, MODE, 1, KIND, 1024, ROWS_ONE>(p, threads(1), 1, sm_count, s);
     if constexpr (MODE == ROWS_BLOCK || (MODE == ROWS_NORM && KIND != ROWS_WHOLE)) {
         if (p.M <= 2 * sm_count) return launch_rows_k<T, MODE, 2, KIND, 1024, ROWS_ONE>(p, threads(2), 1, sm_count, s);
-        const int slot = 16 * rows_arrays(MODE);
-        auto rows = [&](int v, int most) {                       // of a CTA (15: as many as it has barriers)
-            const int fit = most / threads(v) < 15 ? most / threads(v) : 15, turn = 64 * 1024 / (threads(v) * v * slot);
-            return rows_turn(p) && turn < fit ? (turn < 1 ? 1 : turn) : fit;
-        };
-        if (n8 <= 64) return launch_rows_staged<T, MODE, 1, KIND, 768>(p, threads(1), rows(1, 768), sm_count, s);
+        if (n8 <= 64) return launch_rows_staged<T, MODE, 1, KIND, 768>(p, threads(1), 768, sm_count, s);
         // Two groups for each thread rather than four shorten the way from load to store, where as many bytes stay in flight: rows of
         // which a CTA holds one either way (4096 x 16384 102.8 -> 96.5 us; 16384 x 8192 with int8 result, 2 rows rather than 3, 148 -> 164
         // us); short shifted rows, of which four groups would make one or two warps (8190 x 1001 28.2 -> 24.2 us, 8190 x 1501 36.3 -> 32.5,
         // 4090 x 3001 30.7 -> 33.6); single elements, whose addresses do not fit the registers of four groups (4098 x 5001 136 -> 104 us)
         if (KIND == ROWS_SINGLE || n8 > 1536 || (KIND == ROWS_SHIFTED && n8 <= 192))
-            return launch_rows_staged<T, MODE, 2, KIND, 1024>(p, threads(2), rows(2, 1024), sm_count, s);
-        if constexpr (KIND != ROWS_SINGLE) return launch_rows_staged<T, MODE, 4, KIND, 768>(p, threads(4), rows(4, 768), sm_count, s);
+            return launch_rows_staged<T, MODE, 2, KIND, 1024>(p, threads(2), 1024, sm_count, s);
+        if constexpr (KIND != ROWS_SINGLE) return launch_rows_staged<T, MODE, 4, KIND, 768>(p, threads(4), 768, sm_count, s);
         return cudaErrorInvalidValue;
     } else {
         if (n8 <= 64) return launch_rows_k<T, MODE, 2, KIND, 256, ROWS_WARPS>(p, 32, 8, sm_count, s);        // a warp for each row
