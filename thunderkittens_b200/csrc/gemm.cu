@@ -149,8 +149,7 @@ __device__ __forceinline__ void int8_epilogue(uint32_t acc_t, const CUtensorMap*
         if (fp32 && col >= p.N) return;
         uint32_t r[32];
         __syncwarp();
-        tmem_ld_32x32(acc_t + 32 * h, r);
-        tmem_ld_wait();
+        tmem_ld_32x32_wait(acc_t + 32 * h, r);
 #pragma unroll
         for (int i = 0; i < 32; i++) {
             const float c = __shfl_sync(0xffffffffu, col_scale[i % NV], first_lane + (32 * h + i) / NV);

@@ -180,8 +180,7 @@ int8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
             for (int c0 = 32 * half; c0 < p.M; c0 += 64) {                  // (an accumulator has a multiple of 32 columns)
                 uint32_t r[32];
                 __syncwarp();
-                tmem_ld_32x32(tmem_base + (uint32_t(quarter * 32) << 16) + buf * p.acc_cols + c0, r);
-                tmem_ld_wait();
+                tmem_ld_32x32_wait(tmem_base + (uint32_t(quarter * 32) << 16) + buf * p.acc_cols + c0, r);
                 if (mine)
                     typed_out(p, [&](auto* D) {
                         auto* d = D + int64_t(c0) * p.ldd + n;
