@@ -224,7 +224,8 @@ int tkb_fp8_gemm_ex(const void* A, int64_t lda, const void* B, int64_t ldb, void
 
 /* 8-bit integer GEMM with a scale for each token and each output channel:
  *   D[m, n] = A_sc[m] * B_sc[n] * sum_k A[m, k] * B[n, k]
- *   A [M, K], B [N, K] int8, row pitches lda / ldb bytes (0 = K; multiples of 16, 16-byte aligned bases; lda is free when M == 1);
+ *   A [M, K], B [N, K] int8, row pitches lda / ldb bytes (0 = K; multiples of 16, 16-byte aligned bases); a pitch of a single row
+ *   (lda and ldd when M == 1, ldb when N == 1) is not looked at;
  *   A_sc [M], B_sc [N] fp32; D [M, N] of `dtype` (bf16, fp16 or fp32), row pitch ldd elements (0 = N), any alignment.
  *   Any M >= 0, N >= 1, 1 <= K <= 131071 (the sum is exact in int32), odd ones too; M, N <= 2^30.  The sum is converted to fp32,
  *   multiplied by A_sc[m], then by B_sc[n], and rounded to `dtype`: results depend neither on the run nor on the kernel or tile that

@@ -331,15 +331,13 @@ static int int8_gemm_common(const void* A, int64_t lda, const float* A_sc, const
         return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: need M >= 0, N, K >= 1 and M, N <= 2^30 (got %d, %d, %d)", M, N, K);
     if (K > kInt8MaxK) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: K=%d is above %d, where a sum of K products may leave int32", K, kInt8MaxK);
     if (config < TKB_GEMM_DEFAULT || config > TKB_GEMM_SINGLE_N128) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: config %d is not a tile of this format", config);
-    if (lda == 0) lda = K;
-    if (ldb == 0) ldb = K;
-    if (ldd == 0) ldd = N;
+    // a single row has no pitch that anything reads
+    if (lda == 0 || M <= 1) lda = M <= 1 ? (int64_t(K) + 15) / 16 * 16 : K;
+    if (ldb == 0 || N == 1) ldb = N == 1 ? (int64_t(K) + 15) / 16 * 16 : K;
+    if (ldd == 0 || M <= 1) ldd = N;
     if (lda < K || ldb < K || ldd < N) return api_fail(TKB_ERR_BAD_ALIGNMENT, "int8_gemm: lda, ldb must be >= K and ldd >= N");
     if (M == 0) return TKB_OK;
     if (!A || !A_sc || !B || !B_sc || !D) return api_fail(TKB_ERR_INVALID_ARG, "int8_gemm: null pointer");
-    // a single row has no pitch that anything reads
-    if (M == 1) lda = (int64_t(K) + 15) / 16 * 16;
-    if (N == 1) ldb = (int64_t(K) + 15) / 16 * 16;
     if (!aligned16(A) || !aligned16(B) || lda % 16 || ldb % 16)
         return api_fail(TKB_ERR_BAD_ALIGNMENT, "int8_gemm: operand base pointers and row pitches must be multiples of 16 bytes (lda=%lld ldb=%lld); rows of odd K need padded pitches",
                         (long long)lda, (long long)ldb);
