@@ -32,6 +32,19 @@ def test_block_norm_does_not_depend_on_which_outputs_are_asked_for(cuda, lib, M,
     assert torch.equal(got[1][2], got[2][2]) and torch.equal(got[1][3], got[2][3])
 
 
+@pytest.mark.parametrize("M,G,K", [(6, 6, 64), (600, 600, 1000), (600, 4, 1001), (5, 5, 1)])
+def test_block_norm_one_gate_row_expanded(cuda, lib, M, G, K):
+    x, h, w1, w2 = _inputs(M, K, torch.bfloat16, cuda, 17)
+    gate = torch.randn(K, device=cuda).to(torch.bfloat16)
+    out = [[torch.full_like(x, float("nan")) for _ in range(2)] for _ in range(2)]
+    for (R, Y), g in zip(out, (gate, gate.expand(G, K))):
+        _ops().block_norm(h, x, R, w1, g, 0.5, w2, Y, eps=EPS)
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    _check_block(x, h, w1, w2, gate[None], 0.5, *out[1], None, None)
+    with pytest.raises(RuntimeError, match="multiple"):
+        _ops().block_norm(h, x, out[0][0], w1, gate.expand(M + 1, K))
+
+
 def _at(t, off, pitch, guard=7.0):
     """(a view with the values of t whose rows begin `off` elements into rows of `pitch`, its buffer, a mask of what lies outside)."""
     M, K = t.shape

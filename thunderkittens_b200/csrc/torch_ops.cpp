@@ -172,9 +172,15 @@ PyObject* block_norm(PyObject* const* o) {
             gate = vector(o[4], "gate", only(h.dtype), dev, K);
             ldg = K; per = M > 0 ? M : 1;
         } else {
-            const Matrix g = matrix(o[4], "gate", only(h.dtype), dev, -1, K);
-            if (g.n ? M % g.n != 0 || (M > 0 && M < g.n) : M > 0) fail("gate has %d rows, of which %d rows of H are no multiple", g.n, M);
-            gate = g.data; ldg = g.pitch; per = g.n && M >= g.n ? M / g.n : 1;
+            const at::Tensor& t = tensor(o[4], "gate", only(h.dtype), dev, {-1, K});
+            const int n = int(t.size(0));
+            if (n ? M % n != 0 || (M > 0 && M < n) : M > 0) fail("gate has %d rows, of which %d rows of H are no multiple", n, M);
+            if (n > 1 && t.stride(0) == 0 && (t.stride(1) == 1 || K == 1)) {       // one row, expanded
+                gate = t.data_ptr(); ldg = K; per = M > 0 ? M : 1;
+            } else {
+                const Matrix g = matrix(o[4], "gate", only(h.dtype), dev, n, K);
+                gate = g.data; ldg = g.pitch; per = n && M >= n ? M / n : 1;
+            }
         }
     }
     const bool second = o[7] != Py_None || o[8] != Py_None;

@@ -214,6 +214,6 @@ def block_norm(H, X, X_out, W_post=None, gate=None, residual_scale: float = 1.0,
         y = norm(r) * W_pre                               -> Y and / or Y_int8, Y_sc as in rms_norm (W_pre None: left out)
 
     gate is (K,), or (G,K) with M a multiple of G: row i uses gate row i // (M // G), that is one gate for each sequence of a
-    batch, or with G = M one for each token.  X_out may be X."""
+    batch, or with G = M one for each token; one row expanded over G counts as one gate.  X_out may be X."""
     if code := _native().block_norm(H, X, X_out, W_post, gate, residual_scale, W_pre, Y, Y_int8, Y_sc, eps):
         L.check(code)
