@@ -16,7 +16,7 @@ def pytest_configure(config):
 def lib():
     """The product library, built in-tree if needed (nvcc cross-compiles without a GPU)."""
     from thunderkittens_b200 import build, _lib
-    if not os.path.exists(_lib.LIB_PATH):
+    if not (os.path.exists(_lib.LIB_PATH) and os.path.exists(build.TORCH_OPS)):
         build.build()
     return _lib.lib()
 

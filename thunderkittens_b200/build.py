@@ -1,5 +1,6 @@
-"""Builds thunderkittens_b200/libtkb200.so from csrc/*.cu with nvcc for sm_100a, and on top of it the Python module
-thunderkittens_b200/_torch_ops.so from csrc/torch_ops.cpp with the host compiler (in-tree).
+"""Builds thunderkittens_b200/libtkb200.so from csrc/*.cu with nvcc for sm_100a, and on top of it, for the Python and torch that run
+this, the module thunderkittens_b200/_torch_ops.<python's tag>.so from csrc/torch_ops.cpp with the host compiler (in-tree).  Without torch
+or a host compiler the C library is all that is built.
 
     python -m thunderkittens_b200.build [--force] [--verbose]
 
@@ -8,6 +9,7 @@ nvcc cross-compiles without a GPU.  Objects go to thunderkittens_b200/_obj/ (git
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
 import sysconfig
@@ -17,7 +19,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_obj")
 LIB = os.path.join(HERE, "libtkb200.so")
-TORCH_OPS = os.path.join(HERE, "_torch_ops.so")
+TORCH_OPS = os.path.join(HERE, "_torch_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
+CXX = "g++"
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
@@ -68,21 +71,37 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 
 def _build_torch_ops(force: bool) -> None:
+    """The module of the int8 and norm calls; a module that another torch was built with is replaced."""
+    try:
+        import torch
+    except ImportError:
+        torch = None
+    if torch is None or shutil.which(CXX) is None:
+        print(f"{LIB} is built; {TORCH_OPS}, which ops.int8_* and the norms of ops need, is not: {'no torch' if torch is None else 'no ' + CXX}", file=sys.stderr)
+        return
     src = os.path.join(CSRC, "torch_ops.cpp")
     deps = [src, os.path.join(os.path.dirname(HERE), "include", "tkb200.h"), __file__]
-    if not force and os.path.exists(TORCH_OPS) and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_OPS) for d in deps):
+    stamp = os.path.join(OBJ, os.path.basename(TORCH_OPS) + ".torch")                 # the torch that it was built with
+    try:
+        with open(stamp) as f:
+            built_with = f.read()
+    except OSError:
+        built_with = None
+    if not force and built_with == torch.__version__ and os.path.exists(TORCH_OPS) and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_OPS) for d in deps):
         return
-    import torch
     torch_dir = os.path.dirname(torch.__file__)
     include = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], os.path.join(CUDA_HOME, "include")]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DTKB_TORCH_VERSION="{torch.__version__}"',
            *(a for d in include for a in ("-isystem", d)), src, "-o", TORCH_OPS, "-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
            "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError("g++ failed on torch_ops.cpp")
+        raise RuntimeError(f"{CXX} failed on torch_ops.cpp")
+    with open(stamp, "w") as f:
+        f.write(torch.__version__)
 
 
 if __name__ == "__main__":

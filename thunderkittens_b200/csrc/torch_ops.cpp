@@ -220,4 +220,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods,
 
 } // namespace
 
-PyMODINIT_FUNC PyInit__torch_ops() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__torch_ops() {
+    PyObject* const m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", TKB_TORCH_VERSION) != 0) {      // that it was built with
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

@@ -172,11 +172,17 @@ _torch_ops = None
 
 
 def _native():
-    """The module that checks these calls' tensors and launches them; raises if it has not been built."""
+    """The module that checks these calls' tensors and launches them; raises if it has not been built for this Python and torch."""
     global _torch_ops
     if _torch_ops is None:
         L.lib()
-        from . import _torch_ops as module
+        try:
+            from . import _torch_ops as module
+        except ImportError as e:
+            raise ImportError(f"the module of the int8 and norm calls cannot be loaded ({e}): run `python -m thunderkittens_b200.build`") from e
+        if getattr(module, "torch_version", None) != torch.__version__:
+            raise ImportError(f"the module of the int8 and norm calls was built with torch {getattr(module, 'torch_version', '(unknown)')}, "
+                              f"this is {torch.__version__}: run `python -m thunderkittens_b200.build`")
         _torch_ops = module
     return _torch_ops
 
