@@ -150,3 +150,24 @@ def test_quantize_rows_that_begin_anywhere(cuda, lib, M, K, off, dtype):
     codes, steps = quantize64(x)
     assert torch.equal(Q.double(), codes) and torch.equal(sc, steps.float())
     assert bool((qb[qo] == 77).all())
+
+
+def test_row_lengths_in_turn_do_not_ask_the_driver_again(cuda, lib):
+    """A model's hidden and inner rows go through one instance of the kernel; how many CTAs fit is asked for once for each length."""
+    from torch.profiler import ProfilerActivity, profile
+    calls = []
+    for K in (2048, 7168, 5000):
+        x = torch.randn(4, K, device=cuda).to(torch.bfloat16)
+        calls.append((x, torch.empty(4, K, dtype=torch.int8, device=cuda), torch.empty(4, device=cuda)))
+    for c in calls:
+        _ops().int8_quantize(*c)
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CPU, ProfilerActivity.CUDA]) as p:
+        for _ in range(3):
+            for c in calls:
+                _ops().int8_quantize(*c)
+        torch.cuda.synchronize()
+    names = [e.name for e in p.events()]
+    if sum("aunch" in n for n in names) < 9:
+        pytest.skip("the profiler records no runtime calls here")
+    assert not [n for n in names if "Occupancy" in n]
