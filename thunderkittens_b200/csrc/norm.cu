@@ -493,8 +493,11 @@ template <typename T, int MODE, int KIND>
 static cudaError_t launch_rows_m(const RowsParams& p, int sm_count, cudaStream_t s) {
     const int n8 = (p.K + (KIND == ROWS_SHIFTED ? 7 : 0) + 7) / 8;
     auto threads = [&](int v) { return ((n8 + v - 1) / v + 31) / 32 * 32; };
-    if (p.M <= 2 * sm_count && n8 <= 1024) return launch_rows_k<T, MODE, 1, KIND, 1024, ROWS_ONE>(p, threads(1), 1, sm_count, s);
-    if constexpr (MODE == ROWS_BLOCK || (MODE == ROWS_NORM && KIND != ROWS_WHOLE)) {
+    if constexpr (MODE == ROWS_QUANT && KIND == ROWS_SINGLE)         // (only rows that are too long to be shifted)
+        return launch_rows_k<T, MODE, 8, KIND, 1024, ROWS_ONE>(p, threads(8), 1, sm_count, s);
+    else if (p.M <= 2 * sm_count && n8 <= 1024)
+        return launch_rows_k<T, MODE, 1, KIND, 1024, ROWS_ONE>(p, threads(1), 1, sm_count, s);
+    else if constexpr (MODE == ROWS_BLOCK || (MODE == ROWS_NORM && KIND != ROWS_WHOLE)) {
         if (p.M <= 2 * sm_count) return launch_rows_k<T, MODE, 2, KIND, 1024, ROWS_ONE>(p, threads(2), 1, sm_count, s);
         if (n8 <= 64) return launch_rows_staged<T, MODE, 1, KIND, 768>(p, threads(1), 768, sm_count, s);
         // Two groups for each thread rather than four shorten the way from load to store, where as many bytes stay in flight: rows of
