@@ -489,6 +489,11 @@ static cudaError_t launch_rows_staged(const RowsParams& p, int threads, int most
 // the weights pays where a row meets two of them or reaches them unaligned: 16384 x 7168 block_norm 161 -> 156 us, 4098 x 5001 90 ->
 // 52 us, rms_norm 28.7 -> 24.9 us; an aligned rms_norm does better with its weights from L1 and more rows on an SM: 2048 x 8192 12.6
 // against 15.8 us.
+// One row for each CTA (the last branch): groups for each thread so that a CTA has up to 8 warps, 16 for the longest.  In us for rms_norm / with
+// int8 result / int8_quantize, by this rule against others: 16384 x 512 a warp for each row 7.0 / 6.7 / 5.9, a CTA 8.4 / 9.5 / 6.4; 16384 x 2048 1
+// group 27.6 / 31.5 / 17.7, 2 22.6 / 21.2 / 16.9; 16384 x 4096 2 groups 46.0 / 39.9 / 31.4, 1 56.0 / 63.3 / 33.5, 4 46.9 / 34.3 / 31.6; 16384 x
+// 8192 4 groups 90.3 / 66.5 / 61.5, 2 92.4 / 76.4 / 62.5, 8 83.4 / 62.1 / 63.6; 8192 x 16384 4 groups 91.8 / 78.9 / 61.1, 2 92.5 / 84.3 / 69.4,
+// 8 94.3 / 63.7 / 63.9; of few rows (400 x 8192) 4 groups 4.0 / 3.4 / 3.1, 8 4.8 / 3.9 / 3.3.
 template <typename T, int MODE, int KIND>
 static cudaError_t launch_rows_m(const RowsParams& p, int sm_count, cudaStream_t s) {
     const int n8 = (p.K + (KIND == ROWS_SHIFTED ? 7 : 0) + 7) / 8;
